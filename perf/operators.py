@@ -11,7 +11,8 @@ moe       a whole expert layer for one to eight tokens: routing, the chosen unit
 
 How the 4-bit matrices lie in memory is part of the operators' interface: four blocks of 32 elements (128 of a row; a row is
 padded with zeros to whole groups) are 64 bytes, sixteen 32-bit words; word 4 t + b holds elements 8 t .. 8 t + 7 of block b,
-element i of a word in bits 4 i .. 4 i + 3. A block's scale is one byte s, standing for 2^(s - 127); scales lie in block order.
+its elements 0, 2, 4, 6 in bits 0 .. 15 and 1, 3, 5, 7 in bits 16 .. 31, four bits each, from the lowest up. A block's scale is
+one byte s, standing for 2^(s - 127); scales lie in block order.
 """
 import math
 
@@ -135,7 +136,8 @@ def _to_mx4(x):
     size = (torch.round(size / step) * step).clamp(max=6.0)               # torch.round: a tie goes to the even one
     grid = torch.tensor(GRID, dtype=torch.float64, device=x.device)
     code = torch.searchsorted(grid, size) | (torch.signbit(x).long() << 3)
-    code = code.to(torch.uint8).view(rows, groups, 4, 4, 4, 2)             # block, word, byte, nibble
+    code = code.to(torch.uint8).view(rows, groups, 4, 4, 4, 2).transpose(-1, -2)     # block, word, parity, place
+    code = code.reshape(rows, groups, 4, 4, 4, 2)                                    # block, word, byte, half of the byte
     codes = (code[..., 0] | (code[..., 1] << 4)).transpose(2, 3).reshape(rows, groups * 64).contiguous()
     return codes, scales.to(torch.uint8).contiguous()
 
@@ -145,7 +147,8 @@ def _from_mx4(codes, scales, width):
     lead, groups = codes.shape[:-1], codes.shape[-1] // 64
     grid = torch.tensor(GRID + tuple(-g for g in GRID), dtype=torch.float32, device=codes.device)
     code = codes.view(*lead, groups, 4, 4, 4).transpose(-3, -2)            # word, block -> block, word
-    code = torch.stack((code & 15, code >> 4), dim=-1).reshape(*lead, groups * 4, BLOCK)
+    code = torch.stack((code & 15, code >> 4), dim=-1).reshape(*lead, groups * 4, 4, 2, 4)
+    code = code.transpose(-1, -2).reshape(*lead, groups * 4, BLOCK)        # parity, place -> place, parity
     value = grid[code.long()] * _power(scales.long() - 127).float().view(*lead, groups * 4, 1)
     return value.view(*lead, groups * GROUP)[..., :width]
 
@@ -400,7 +403,7 @@ def _exact_values(codes, scales, width):
     for b in range(4):
         for t in range(4):
             for i in range(8):
-                code = (words[:, :, 4 * t + b] >> (4 * i)) & 15
+                code = (words[:, :, 4 * t + b] >> (4 * (i // 2) + 16 * (i % 2))) & 15
                 e, m = (code >> 1) & 3, (code & 1).double()
                 size = torch.where(e == 0, 0.5 * m, 2.0 ** (e.double() - 1) * (1 + 0.5 * m))
                 out[:, :, b, 8 * t + i] = torch.where(code >= 8, -size, size)
