@@ -1,0 +1,29 @@
+// Microscaled 4-bit matrices: how they lie in memory, and the pieces that the kernels which read them share.
+//
+// 32 neighbouring elements of a row, a block, share a power of two; an element is sign, two bits of exponent and one of
+// mantissa (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6). Four blocks, a group of 128 elements, are sixteen 32-bit words: word 4 t + b holds
+// elements 8 t .. 8 t + 7 of block b, so that one 16-byte load gives lane t of four its eighth of every block of the group. In a word
+// elements 0, 2, 4, 6 lie in bits 0 .. 15 and 1, 3, 5, 7 in bits 16 .. 31, so that one mask cuts out two neighbours at once. A row is
+// padded with zeros to whole groups. A block's scale is a byte s for 2^(s - 127), four bytes a group; s = 255 marks a block
+// that had no finite numbers.
+#pragma once
+#include <stdint.h>
+
+namespace mx4 {
+constexpr int BLOCK = 32, GROUP = 128, GROUP_BYTES = 64;
+
+// The eight elements of a word as bfloat16 pairs (0,1) (2,3) (4,5) (6,7), each element times 2^-126: exponent and mantissa
+// bits moved to the low end of bfloat16's exponent. 0.5 becomes a subnormal, which the tensor cores take as it is.
+__device__ __forceinline__ void pairs(uint32_t w, uint32_t* v) {
+    constexpr uint32_t SIGN = 0x80008000u, SIZE = 0x01C001C0u;
+    v[0] = ((w << 12) & SIGN) | ((w << 6) & SIZE);
+    v[1] = ((w << 8) & SIGN) | ((w << 2) & SIZE);
+    v[2] = ((w << 4) & SIGN) | ((w >> 2) & SIZE);
+    v[3] = (w & SIGN) | ((w >> 6) & SIZE);
+}
+// 2^(s - 127) of block b of a group's four scale bytes. s = 0 counts as zero (its elements are below 2^-124); s = 255 as infinity.
+__device__ __forceinline__ float scale(uint32_t four, int b) {
+    const uint32_t moved = b == 0 ? four << 23 : b == 1 ? four << 15 : b == 2 ? four << 7 : four >> 1;
+    return __uint_as_float(moved & 0x7f800000u);
+}
+}  // namespace mx4
