@@ -23,6 +23,7 @@
 // The order of an expert's rows among themselves depends on the order in which threads arrive; no value depends
 // on it, since every row is computed by itself and the sum over a token's experts runs in the order of its choices.
 #include "common.cuh"
+#include "route_choice.cuh"
 
 namespace {
 constexpr int ROUTE_THREADS = 1024;
@@ -195,84 +196,15 @@ route_by_score_kernel(const T* y, int ldy, const T* router, int ldr, int width, 
             value[e] = z;                        // the logits; the first warp turns them into scores
             continue;
         }
-        const float s = 1.0f / (1.0f + expf(-z));
-        if (e < n_experts) {
-            value[e] = s;
-            // where nothing is added to the scores the logits choose: their order is the scores', which run together near one
-            score[e] = correction ? s + correction[e] : (groups > 1 ? s : z);
-        } else if (shared_scale) shared_scale[t] = s;
+        if (e < n_experts) dd_sigmoid_score(z, e, correction, groups, value, score);
+        else if (shared_scale) shared_scale[t] = 1.0f / (1.0f + expf(-z));
     }
     if (threadIdx.x == 0 && shared_scale && gate_row < 0) shared_scale[t] = 1.0f;
     __syncthreads();
     if (warp) return;
     __syncwarp();
-    constexpr float NONE = -3.0e38f;             // below every score: struck out
-    if (softmax) {
-        float top_z = NONE, total = 0.f;
-        for (int e = lane; e < n_experts; e += 32) top_z = fmaxf(top_z, value[e]);
-        top_z = dd_warp_max(top_z);
-        for (int e = lane; e < n_experts; e += 32) total += expf(value[e] - top_z);
-        total = dd_warp_sum(total);
-        for (int e = lane; e < n_experts; e += 32) {
-            const float s = expf(value[e] - top_z) / total;
-            value[e] = s;
-            score[e] = correction ? s + correction[e] : s;
-        }
-        __syncwarp();
-    }
-    const int per = n_experts / groups;
-    if (groups > 1) {
-        for (int g = lane; g < groups; g += 32) {
-            float best = NONE, second = NONE;
-            for (int i = 0; i < per; ++i) {
-                const float s = score[g * per + i];
-                if (s > best) { second = best; best = s; }
-                else if (s > second) second = s;
-            }
-            worth[g] = best + (per > 1 ? second : 0.f);
-        }
-        __syncwarp();
-        // keep the worthiest runs: the others' scores are struck out
-        // (a kept run's worth becomes infinite and is passed over from then on)
-        for (int round = 0; round < keep; ++round) {
-            float best = -INFINITY;
-            int at = 0x7fffffff;
-            for (int g = lane; g < groups; g += 32)
-                if (worth[g] > best && worth[g] < INFINITY) { best = worth[g]; at = g; }
-            for (int o = 16; o > 0; o >>= 1) {
-                const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-                const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-                if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-            }
-            if (lane == 0 && at < groups) worth[at] = INFINITY;     // marked as kept
-            __syncwarp();
-        }
-        for (int e = lane; e < n_experts; e += 32)
-            if (worth[e / per] != INFINITY) score[e] = NONE;
-        __syncwarp();
-    }
-    float sum = 0.f;                             // of the chosen scores, in the order of the choice (lane 0)
-    for (int k = 0; k < top; ++k) {
-        float best = NONE;
-        int at = 0x7fffffff;
-        for (int e = lane; e < n_experts; e += 32)
-            if (score[e] > best) { best = score[e]; at = e; }
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-            if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-        }
-        if (lane == 0) {
-            chosen[(size_t)t * top + k] = at < n_experts ? at : -1;
-            const float s = at < n_experts ? value[at] : 0.f;
-            pair_weight[(size_t)t * top + k] = s * weight_scale;
-            sum += s;
-            if (at < n_experts) score[at] = NONE;
-        }
-        __syncwarp();
-    }
-    if (renormalize && lane == 0)
-        for (int k = 0; k < top; ++k) pair_weight[(size_t)t * top + k] /= sum + 1e-20f;
+    dd_choose_experts(score, value, worth, n_experts, top, groups, keep, weight_scale, softmax, correction, renormalize,
+                      chosen + (size_t)t * top, pair_weight + (size_t)t * top);
 }
 
 template <typename T>

@@ -104,6 +104,7 @@ _SIGNATURES = {
         "dd_post_norm": [_c_void, _c_void, _c_void, _c_float, _c_float, _c_void, _c_int, _c_void, _c_float, _c_float, _c_void, _c_int,
                          _c_int, _c_int, _c_void],
         "dd_round_rows": [_c_void, _c_void, ctypes.c_longlong, _c_void],
+        "dd_moe_tokens": [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
         "dd_mx4_quantize": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_int, _c_void],
         "dd_mx4_values": [_c_void, _c_void, ctypes.c_longlong, _c_int, _c_void, _c_int, _c_void],
         "dd_gemm_mx4_rows": [_c_void, _c_int] + [_c_void] * 4 + [_c_int, _c_void] + [_c_int] * 6 + [_c_void],
@@ -173,6 +174,8 @@ def library(name):
         for fn, args in _SIGNATURES[name].items():
             f = getattr(lib, fn)
             f.argtypes, f.restype = args, _c_int
+        if name == "core":
+            lib.dd_moe_tokens_scratch.argtypes, lib.dd_moe_tokens_scratch.restype = [_c_void, _c_int], ctypes.c_longlong
         _libs[name] = lib
         return lib
 
@@ -1515,6 +1518,116 @@ def combine_rows(y, pair_row, stream_rows, top, weight, pair_weight=None, own=No
           stream_rows.shape[0], stream_rows.shape[1], int(top), float(weight), _stream(), _ptr(pair_weight, "pair_weight"),
           _ptr(own, "own"), F32 if own is None else _dt(own.dtype))
     return stream_rows
+
+
+# ---------------------------------------------------------------- expert layers for a few tokens
+
+MOE_TOKENS, MOE_TOP, MOE_OUTPUTS = 8, 16, 256        # most tokens, choices a token, and router rows of moe_tokens
+
+
+class _ExpertLayer(ctypes.Structure):                # csrc/moe_tokens.cu: DdExpertLayer
+    _fields_ = [(n, _c_void) for n in ("gate_up", "gate_up_scales", "down", "down_scales", "shared_gate_up", "shared_gate_up_scales",
+                                       "shared_down", "shared_down_scales", "router", "table", "correction")] + \
+               [(n, _c_int) for n in ("kind", "width", "inner", "experts", "top", "vocab", "identity", "gated", "form", "act", "softmax",
+                                      "groups", "keep", "renormalize", "weight_input", "shared_inner", "shared_form", "shared_gate",
+                                      "router_stride")] + \
+               [(n, _c_float) for n in ("limit", "alpha", "shared_limit", "shared_alpha", "weight_scale")]
+
+
+class ExpertLayer:
+    """The tensors and options of an expert layer, as moe_tokens takes them (built once; it keeps the tensors).
+
+    gate_up [E, 2 * inner, width] (gate rows, then up rows; plain units: [E, inner, width]) and down [E, width, inner]: float32,
+    bfloat16, or Mx4Matrix stacks (the rows are then bfloat16). gated: (limit, alpha, form) as gemm_grouped_tcgen05, or None with
+    ``activation`` for plain units. Routing: ``table`` int32 [vocab, top], every choice weighing weight_scale / top; or ``router``
+    [E + identity (+ 1), width] in the rows' type with the options of route_by_score (with ``shared_gate`` its last row is the
+    shared unit's gate vector). Outputs E .. E + identity - 1 are the token's own row. weight_input: a choice's weight multiplies the
+    unit's product before its activation instead of its output (plain units without identity outputs). shared: (gate_up
+    [2 * n, width], down [width, n]) of a unit that every token uses, of the experts' kind, shared_gated its form."""
+
+    def __init__(self, gate_up, down, top, *, gated=None, activation=None, router=None, table=None, softmax=False, groups=1, keep=1,
+                 weight_scale=1.0, correction=None, renormalize=False, identity=0, weight_input=False, shared=None, shared_gated=None,
+                 shared_gate=False):
+        four = isinstance(gate_up, Mx4Matrix)
+        if gate_up.dim() != 3 or down.dim() != 3 or isinstance(down, Mx4Matrix) != four:
+            raise KernelError("expert layer: gate_up and down must be stacks of matrices of one kind")
+        E, width, inner = gate_up.shape[0], gate_up.shape[2], down.shape[2]
+        halves = 2 if gated else 1
+        if tuple(gate_up.shape) != (E, halves * inner, width) or tuple(down.shape) != (E, width, inner):
+            raise KernelError(f"expert layer: gate_up {tuple(gate_up.shape)} does not fit down {tuple(down.shape)}")
+        self.dtype = torch.bfloat16 if four else gate_up.dtype
+        matrices = [gate_up, down, *(shared or ())]
+        if any(isinstance(m, Mx4Matrix) != four or (not four and (m.dtype != self.dtype or not m.is_contiguous())) for m in matrices) or \
+                self.dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError("expert layer: matrices must be contiguous and all float32, all bfloat16 or all in 4 bits")
+        outputs = E + identity
+        if not 0 < top <= min(outputs, MOE_TOP) or identity < 0 or outputs + bool(shared_gate) > MOE_OUTPUTS:
+            raise KernelError(f"expert layer: {top} of {outputs} experts per token (at most {MOE_TOP} of {MOE_OUTPUTS})")
+        if (router is None) == (table is None):
+            raise KernelError("expert layer: a router or a table")
+        if table is not None and (table.dim() != 2 or table.shape[1] != top or table.dtype != torch.int32 or not table.is_contiguous() or identity
+                                  or shared_gate or weight_input):
+            raise KernelError(f"expert layer: the table must be int32 [vocab, {top}] (and goes with plain sums of units)")
+        if router is not None and (router.dim() != 2 or tuple(router.shape) != (outputs + bool(shared_gate), width) or router.dtype != self.dtype
+                                   or router.stride(1) != 1):
+            raise KernelError(f"expert layer: router {tuple(router.shape)} {router.dtype} does not fit {outputs} experts over {width} {self.dtype}")
+        if correction is not None and (correction.numel() != outputs or correction.dtype != torch.float32 or not correction.is_contiguous()):
+            raise KernelError("expert layer: the correction must be float32 [experts]")
+        if groups <= 0 or outputs % groups or not 0 < keep <= groups or top > outputs // groups * keep:
+            raise KernelError(f"expert layer: {top} of {outputs} experts in {groups} groups of which {keep} stay")
+        if bool(gated) == (activation is not None) or (weight_input and (gated or identity)) or (gated and gated[2] not in GATED_FORMS) or \
+                (activation is not None and activation not in ACTIVATIONS):
+            raise KernelError("expert layer: gated units, or plain ones with an activation (only these with weights on their inputs)")
+        if shared_gate and not shared:
+            raise KernelError("expert layer: a shared unit's gate without a shared unit")
+        if shared and (shared[0].shape[0] != 2 * shared[1].shape[1] or shared[0].shape[1] != width or shared[1].shape[0] != width
+                       or not shared_gated or shared_gated[2] not in GATED_FORMS):
+            raise KernelError(f"expert layer: shared unit {tuple(shared[0].shape)}, {tuple(shared[1].shape)} of width {width}")
+        self.width, self.top, self.by_table, self.tensors = width, top, table is not None, (gate_up, down, router, table, correction, shared)
+        pair = lambda m, what: (_ptr(m.codes, what), _ptr(m.scales, what)) if four else (_ptr(m, what), None)  # noqa: E731
+        limit, alpha, form = gated or (0.0, 0.0, "clamped_swish")
+        s_limit, s_alpha, s_form = shared_gated if shared else (0.0, 0.0, "clamped_swish")
+        raw = self._raw = _ExpertLayer(
+            *pair(gate_up, "gate_up"), *pair(down, "down"), *(pair(shared[0], "shared") if shared else (None, None)),
+            *(pair(shared[1], "shared") if shared else (None, None)), _ptr(router, "router"), _ptr(table, "table"),
+            _ptr(correction, "correction"), 2 if four else (0 if self.dtype == torch.float32 else 1), width, inner, E, top,
+            table.shape[0] if table is not None else 0, identity, 1 if gated else 0, GATED_FORMS[form], ACTIVATIONS[activation],
+            1 if softmax else 0, groups, keep, 1 if renormalize else 0, 1 if weight_input else 0, shared[1].shape[1] if shared else 0,
+            GATED_FORMS[s_form], 1 if shared_gate else 0, router.stride(0) if router is not None else 0, float(limit), float(alpha),
+            float(s_limit), float(s_alpha), float(weight_scale) / (top if table is not None else 1))
+        self.device_index = gate_up.device.index
+        if any(t is not None and t.device.index != self.device_index for t in (router, table, correction)) or \
+                any(m.device.index != self.device_index for m in matrices):
+            raise KernelError("expert layer: its tensors are on more than one device")
+        self._at = ctypes.addressof(raw)
+        self._scratch = [0] + [int(library("core").dd_moe_tokens_scratch(self._at, t)) for t in range(1, MOE_TOKENS + 1)]
+
+
+def moe_tokens(layer, y, residual=None, ids=None, out=None):
+    """A whole expert layer for one to MOE_TOKENS tokens in two kernels: routing, the chosen units, the shared unit, the weighted
+    sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the layer's dtype; ids int32 [T] for a layer by
+    table; out float32 (residual itself may be given). Sums are float32; a hidden row meets the down matrix as float32, in
+    bfloat16 layers as two bfloat16 terms. An expert or token id out of range sets error bit 1 and is left out."""
+    T = y.shape[0]
+    if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > MOE_TOKENS:
+        raise KernelError(f"moe_tokens: rows {tuple(y.shape)} {y.dtype} do not fit a layer of width {layer.width} {layer.dtype} "
+                          f"(at most {MOE_TOKENS} rows)")
+    if layer.by_table != (ids is not None) or (ids is not None and (ids.numel() != T or ids.dtype != torch.int32 or not ids.is_contiguous())):
+        raise KernelError("moe_tokens: a layer by table wants int32 token ids, one a row, and no other does")
+    _check_epilogue("moe_tokens", T, layer.width, None, residual, out)
+    pointer = _ptr(y, "y")
+    _here(y, residual, ids, out)
+    if layer.device_index != y.get_device():
+        raise KernelError(f"moe_tokens: the layer is on cuda:{layer.device_index}, its rows on {y.device}")
+    if out is None:
+        out = torch.empty((T, layer.width), dtype=torch.float32, device=y.device)
+    if T == 0:
+        return out
+    scratch = torch.empty(layer._scratch[T], dtype=torch.uint8, device=y.device)
+    _call(library("core"), "dd_moe_tokens", layer._at, pointer, y.stride(0), _ptr(residual, "residual", torch.float32),
+          0 if residual is None else residual.stride(0), _ptr(out, "out", torch.float32), out.stride(0), _ptr(ids, "ids"), T, scratch.data_ptr(),
+          sm_count(y.device), _ptr(error_flag(y.device)), _stream(), n_kernels=2)
+    return out
 
 
 # ---------------------------------------------------------------- microscaled 4-bit matrices

@@ -58,3 +58,37 @@ def test_plain_quantisation():
     codes, scales = packed(values, marks)
     word = int.from_bytes(bytes(codes[0, :4].tolist()), "little")
     assert word & 15 == 7 and word >> 16 & 15 == 6 and word >> 4 & 15 == 8 + 4 and scales[0, :2].tolist() == [127, 123]
+
+
+# ------------------------------------------------------------------ expert layers
+
+def matrices(E=4, inner=8, width=16, halves=2, dtype=torch.float32):
+    return torch.zeros(E, halves * inner, width, dtype=dtype), torch.zeros(E, width, inner, dtype=dtype)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(top=5), "experts per token"), (dict(top=0), "experts per token"), (dict(router=None), "a router or a table"),
+    (dict(table=torch.zeros(9, 2, dtype=torch.int32)), "a router or a table"), (dict(router=torch.zeros(5, 16)), "router"),
+    (dict(router=torch.zeros(4, 16, dtype=torch.bfloat16)), "router"), (dict(router=None, table=torch.zeros(9, 2)), "table"),
+    (dict(groups=3), "groups"), (dict(groups=2, keep=3), "groups"), (dict(top=3, groups=2, keep=1), "groups"), (dict(gated=None), "does not fit"),
+    (dict(activation="relu2"), "gated"), (dict(weight_input=True), "gated"), (dict(gated=(1.0, 1.0, "other")), "gated"),
+    (dict(shared_gate=True, router=torch.zeros(5, 16)), "shared"), (dict(correction=torch.zeros(3)), "correction"),
+    (dict(shared=(torch.zeros(12, 16), torch.zeros(16, 8)), shared_gated=(1.0, 1.0, "silu")), "shared"),
+    (dict(identity=300, router=torch.zeros(304, 16)), "experts per token")])
+def test_expert_layer_refusals(change, match):
+    gate_up, down = matrices()
+    options = dict(top=2, gated=(7.0, 1.702, "silu"), router=torch.zeros(4, 16))
+    options.update(change)
+    with pytest.raises(kernels.KernelError, match=match):
+        kernels.ExpertLayer(gate_up, down, options.pop("top"), **options)
+
+
+def test_expert_layer_matrices():
+    gate_up, down = matrices()
+    good = dict(gated=(7.0, 1.702, "silu"), router=torch.zeros(4, 16))
+    for a, b in ((gate_up[:3], down), (gate_up[:, :8], down), (gate_up.bfloat16(), down), (gate_up.half(), down.half()), (gate_up[0], down[0]),
+                 (gate_up, down.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(kernels.KernelError, match="expert layer"):
+            kernels.ExpertLayer(a, b, 2, **good)
+    with pytest.raises(kernels.KernelError, match="CUDA"):
+        kernels.ExpertLayer(gate_up, down, 2, **good)
