@@ -1,0 +1,310 @@
+// Products with microscaled 4-bit matrices (mx4.cuh) for many rows, on the 5th-generation tensor cores:
+//
+//     out[r, n] = act(scale[r] * sum_k X[r, k] W[group(tile of r)][n, k] + bias[n]) (+ residual[r, n])
+//
+// X bfloat16 in row tiles, W one matrix or a stack of them of which a tile meets one; or, DUAL, the gated unit of two such products
+// (N gate rows, then N up rows a group), as gemm_grouped_tcgen05.cu does it for bfloat16 matrices.
+//
+// An element times its block's scale is a bfloat16 number exactly, so the weights become bfloat16 on their way to the tensor
+// cores and lose nothing: computed transposed, D^T = W X^T, 128 weight rows are the lanes of the accumulator, and W is the operand
+// that tcgen05.mma reads from tensor memory. A thread owns a row: it takes 128 elements (64 bytes, fetched by TMA) and their
+// four scales, and stores 64 pairs into its lane's columns; eight warps do nothing else until the epilogue. Two elements cost two
+// shifts, two masks and a multiplication, 2.4 operations an element with the store: 128 x 128 elements take four schedulers about
+// 400 clocks, the instructions that use them 4 T for a tile of T rows. So T = 128 where there are rows enough.
+//
+// Rings: X (64 k a stage, TMA -> MMA), codes (128 k, TMA -> the eight warps), W in tensor memory (64 k, warps -> MMA). Without DUAL
+// the two sets of four warps take groups of 128 k in turn, with it one set the gate's and one the up rows. Every wait is bounded.
+#include "common.cuh"
+#include "mx4.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+constexpr int BM = 128, XK = 64, UMMA_K = 16, DEQUANT_WARPS = 8, THREADS = (DEQUANT_WARPS + 2) * 32;
+constexpr int CODE_BYTES = BM * mx4::GROUP_BYTES;
+
+struct Mx4Params {
+    const uint32_t* scales;      // [groups * rows_per_group][K groups]
+    const int* tile_group;       // [row tiles] or null (group 0)
+    const float* bias;           // [N] or null
+    const float* residual;       // [rows, ldr] or null; may be out
+    const float* row_scale;      // [rows] or null
+    void* out;                   // [rows, ldo]
+    int* error_flag;
+    int rows, N, K, k_groups, rows_per_group, ldr, ldo, out_dtype, act, form;
+    float limit, alpha;
+};
+
+template <int T, bool DUAL> struct Mx4Config {
+    static constexpr int X_BYTES = T * XK * 2;
+    static constexpr int W_BYTES = (DUAL ? 2 : 1) * CODE_BYTES;
+    static constexpr int W_STAGES = DUAL ? 2 : 3;
+    static constexpr int X_FIT = (108 * 1024 - W_STAGES * W_BYTES) / X_BYTES;
+    static constexpr int X_STAGES = X_FIT < 8 ? X_FIT : 8;
+    static constexpr int A_STAGES = DUAL ? 2 : 4;                    // of 32 columns (64 k), twice that with DUAL
+    static constexpr int ACC_COLS = (DUAL ? 2 : 1) * T;
+    static constexpr int A_COLS = 128;
+    static constexpr int WANTED = ACC_COLS + A_COLS;
+    static constexpr int TMEM_COLS = WANTED <= 256 ? 256 : 512;
+    static constexpr int BLOCKS = TMEM_COLS == 256 ? 2 : 1;          // an SM
+    static constexpr int BARRIERS = 2 * (X_STAGES + W_STAGES + A_STAGES) + 1;
+    static constexpr int SMEM_BYTES = X_STAGES * X_BYTES + W_STAGES * W_BYTES + 1024 + BARRIERS * 8 + 16;
+};
+
+__device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// The factor of a block's pairs (mx4::pairs): 2^126 * 2^(s - 127), twice in a register; above 2^127 what is missing comes later.
+__device__ __forceinline__ uint32_t pair_factor(uint32_t s) {
+    const uint32_t bits = s == 0 ? 0u : s == 255 ? 0x7fc0u : (min(s, 128u) + 126u) << 7;
+    return bits | (bits << 16);
+}
+
+template <int T, bool DUAL>
+__global__ void __launch_bounds__(THREADS, Mx4Config<T, DUAL>::BLOCKS)
+gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Mx4Params p) {
+    using C = Mx4Config<T, DUAL>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* x_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* w_tiles = x_tiles + C::X_STAGES * C::X_BYTES;
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(w_tiles + C::W_STAGES * C::W_BYTES);
+    uint64_t* x_empty = x_full + C::X_STAGES;
+    uint64_t* w_full = x_empty + C::X_STAGES;
+    uint64_t* w_empty = w_full + C::W_STAGES;
+    uint64_t* a_full = w_empty + C::W_STAGES;
+    uint64_t* a_empty = a_full + C::A_STAGES;
+    uint64_t* acc_bar = a_empty + C::A_STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::X_STAGES; ++s) { tc::mbar_init(&x_full[s], 1); tc::mbar_init(&x_empty[s], 1); }
+        for (int s = 0; s < C::W_STAGES; ++s) { tc::mbar_init(&w_full[s], 1); tc::mbar_init(&w_empty[s], DUAL ? 8 : 4); }
+        for (int s = 0; s < C::A_STAGES; ++s) { tc::mbar_init(&a_full[s], DUAL ? 8 : 4); tc::mbar_init(&a_empty[s], 1); }
+        tc::mbar_init(acc_bar, 1);
+        *abort_flag = 0;
+        tc::fence_barrier_init();
+        tc::fence_proxy_async();
+    }
+    if (warp == DEQUANT_WARPS + 1) {
+        tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot, tmem_a = tmem + C::ACC_COLS;
+    dd_launch_dependents();
+    dd_grid_wait();              // the tile's group and the rows are earlier kernels' results
+
+    const int n0 = blockIdx.x * BM, row0 = blockIdx.y * T;
+    const int group = p.tile_group ? p.tile_group[blockIdx.y] : 0;
+    const int kgroups = p.k_groups, kblocks = (p.K + XK - 1) / XK;
+    if (group >= 0) {
+        if (warp == DEQUANT_WARPS) {
+            if (tc::elect_one()) {
+                tc::prefetch_tensormap(&map_w);
+                tc::prefetch_tensormap(&map_x);
+                const int w_row = group * p.rows_per_group + n0;
+                bool ok = true;
+                for (int i = 0; i < kgroups && ok; ++i) {
+                    const int s = i % C::W_STAGES;
+                    if (!tc::mbar_wait(&w_empty[s], ((i / C::W_STAGES) & 1) ^ 1, abort_flag)) break;
+                    tc::mbar_expect_tx(&w_full[s], C::W_BYTES);
+                    tc::tma_load_2d(w_tiles + s * C::W_BYTES, &map_w, i * mx4::GROUP_BYTES, w_row, &w_full[s]);
+                    if (DUAL) tc::tma_load_2d(w_tiles + s * C::W_BYTES + CODE_BYTES, &map_w, i * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
+                    for (int h = 2 * i; h < min(2 * i + 2, kblocks); ++h) {
+                        const int x = h % C::X_STAGES;
+                        if (!tc::mbar_wait(&x_empty[x], ((h / C::X_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        tc::mbar_expect_tx(&x_full[x], C::X_BYTES);
+                        tc::tma_load_2d(x_tiles + x * C::X_BYTES, &map_x, h * XK, row0, &x_full[x]);
+                    }
+                }
+            }
+        } else if (warp == DEQUANT_WARPS + 1) {
+            if (tc::elect_one()) {
+                constexpr uint32_t idesc = tc::idesc_bf16_f32(BM, T);
+                bool ok = true;
+                for (int h = 0; h < kblocks; ++h) {
+                    const int x = h % C::X_STAGES, a = h % C::A_STAGES;
+                    if (!tc::mbar_wait(&x_full[x], (h / C::X_STAGES) & 1, abort_flag) ||
+                        !tc::mbar_wait(&a_full[a], (h / C::A_STAGES) & 1, abort_flag)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    const uint32_t x_addr = tc::smem_u32(x_tiles + x * C::X_BYTES);
+                    const uint32_t from = tmem_a + a * (DUAL ? 64 : 32);
+#pragma unroll
+                    for (int k = 0; k < XK / UMMA_K; ++k) {
+                        const uint64_t dx = tc::smem_desc_sw128(x_addr + k * UMMA_K * 2);
+                        tc::mma_bf16_a_tmem(tmem, from + k * (UMMA_K / 2), dx, idesc, (h > 0 || k > 0) ? 1u : 0u);
+                        if (DUAL) tc::mma_bf16_a_tmem(tmem + T, from + 32 + k * (UMMA_K / 2), dx, idesc, (h > 0 || k > 0) ? 1u : 0u);
+                    }
+                    tc::mma_commit(&x_empty[x]);
+                    tc::mma_commit(&a_empty[a]);
+                }
+                if (ok) tc::mma_commit(acc_bar);
+            }
+        } else {
+            // warp w may touch lanes 32 * (w % 4) .. + 31 of tensor memory; a thread owns a row of the matrix
+            const int quarter = warp & 3, set = warp >> 2, row = quarter * 32 + lane;
+            const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
+            const size_t w_row = (size_t)group * p.rows_per_group + (DUAL && set ? p.N : 0) + min(n0 + row, p.N - 1);
+            const uint32_t* scales = p.scales + w_row * kgroups;
+            constexpr int STEP = DUAL ? 1 : 2;
+            const int first = DUAL ? 0 : set;
+            uint32_t four = first < kgroups ? __ldg(scales + first) : 0u;
+            bool ok = true;
+            for (int i = first; i < kgroups && ok; i += STEP) {
+                const uint32_t by = four;
+                if (i + STEP < kgroups) four = __ldg(scales + i + STEP);
+                const int s = i % C::W_STAGES;
+                if (!tc::mbar_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
+                // a row is 64 bytes under the 64-byte swizzle: 16-byte piece t lies at t ^ (row / 2 % 4)
+                const uint4* from = reinterpret_cast<const uint4*>(w_tiles + s * C::W_BYTES + (DUAL ? set * CODE_BYTES : 0) + row * mx4::GROUP_BYTES);
+                uint32_t words[4][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint4 v = from[t ^ ((row >> 1) & 3)];
+                    words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&w_empty[s]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int h = 2 * i + half, a = h % C::A_STAGES;
+                    if (h >= kblocks) break;
+                    uint32_t r[32];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t scale = (by >> (16 * half + 8 * b)) & 255u, factor = pair_factor(scale);
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            mx4::pairs(words[t][2 * half + b], r + b * 16 + t * 4);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor);
+                        }
+                        if (scale > 128 && scale < 255) {
+                            const uint32_t more = ((scale - 1) << 7) * 0x10001u;             // 2^(s - 128)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) r[b * 16 + j] = mul_pair(r[b * 16 + j], more);
+                        }
+                    }
+                    if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    tc::tmem_st_x32(tmem_a + lane_part + a * (DUAL ? 64 : 32) + (DUAL ? set * 32 : 0), r);
+                    tc::tmem_st_wait();
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&a_full[a]);
+                }
+            }
+            // epilogue: the two sets share the columns
+            const int n = n0 + row;
+            if (tc::mbar_wait(acc_bar, 0, abort_flag)) {
+                tc::fence_after_sync();
+                const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+#pragma unroll 1
+                for (int c0 = set * (T / 2); c0 < (set + 1) * (T / 2); c0 += 8) {
+                    uint32_t g[8], u[8];
+                    tc::tmem_ld_x8(tmem + lane_part + c0, g);
+                    if (DUAL) tc::tmem_ld_x8(tmem + lane_part + T + c0, u);
+                    tc::tmem_ld_wait();
+                    if (n < p.N) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = row0 + c0 + j;
+                            if (r >= p.rows) break;
+                            float v = __uint_as_float(g[j]);
+                            if (DUAL) v = dd_gated_value<true>(v, __uint_as_float(u[j]), p.form, p.limit, p.alpha);
+                            else v = dd_activation((p.row_scale ? v * p.row_scale[r] : v) + bias, p.act);
+                            if (p.residual) v += p.residual[(size_t)r * p.ldr + n];
+                            const size_t at = (size_t)r * p.ldo + n;
+                            if (p.out_dtype == DD_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+                            else reinterpret_cast<float*>(p.out)[at] = v;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 8);
+    if (warp == DEQUANT_WARPS + 1) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int mx4_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long width, long long row_bytes, int box_width,
+            int box_rows, CUtensorMapSwizzle swizzle, const char* what) {
+    static EncodeTiled enc = nullptr;
+    if (!enc) {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            enc = reinterpret_cast<EncodeTiled>(sym);
+    }
+    if (!enc) return dd_fail("dd_gemm_mx4: cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {(cuuint32_t)box_width, (cuuint32_t)box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return dd_fail("dd_gemm_mx4: cannot describe %s to TMA (driver error %d)", what, (int)r);
+    return 0;
+}
+
+template <int T, bool DUAL>
+int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, cudaStream_t s) {
+    using C = Mx4Config<T, DUAL>;
+    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
+    dd_launch(gemm_mx4_kernel<T, DUAL>, dim3(dd_ceil_div(p.N, BM), dd_ceil_div(p.rows, T)), dim3(THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);
+    return dd_check_launch("dd_gemm_mx4");
+}
+}  // namespace
+
+// X [rows, K] bf16 (row stride ldx) in tiles of `tile` rows (16, 32, 64 or 128); codes, scales: `groups` 4-bit matrices of
+// rows_per_group rows of K; tile_group: device array [rows / tile] (a negative group's tile is skipped), or null: one matrix for
+// all rows, of which the last tile may hold fewer. dual == 0: rows_per_group == N, act(row_scale * sum + bias) + residual; dual != 0:
+// rows_per_group == 2 N, the gated unit. out: [rows, N] bf16 or f32, row stride ldo.
+DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* scales, int groups, int rows_per_group, const int* tile_group,
+                       const float* bias, const float* residual, int ldr, const float* row_scale, void* out, int ldo, int rows, int N, int K,
+                       int tile, int dual, float limit, float alpha, int form, int act, int out_dtype, int* error_flag, void* stream) {
+    if (rows <= 0 || N <= 0) return 0;
+    if (K <= 0 || K % 8 || ldx % 8) return dd_fail("dd_gemm_mx4: K=%d and the row stride %d must be multiples of 8 (TMA needs 16-byte rows)", K, ldx);
+    if (((uintptr_t)X & 15) || ((uintptr_t)codes & 15)) return dd_fail("dd_gemm_mx4: operands must be 16-byte aligned");
+    if (out_dtype != DD_BF16 && out_dtype != DD_F32) return dd_fail("dd_gemm_mx4: unknown output dtype %d", out_dtype);
+    if (tile <= 0 || (tile_group && rows % tile) || dd_ceil_div(rows, tile) > 65535) return dd_fail("dd_gemm_mx4: %d rows in tiles of %d", rows, tile);
+    if (groups <= 0 || (groups > 1 && !tile_group) || rows_per_group != (dual ? 2 * N : N))
+        return dd_fail("dd_gemm_mx4: %d groups of %d rows do not fit N=%d", groups, rows_per_group, N);
+    Mx4Params p;
+    p.scales = (const uint32_t*)scales; p.tile_group = tile_group; p.bias = bias; p.residual = residual; p.row_scale = row_scale; p.out = out;
+    p.error_flag = error_flag; p.rows = rows; p.N = N; p.K = K; p.k_groups = dd_ceil_div(K, mx4::GROUP); p.rows_per_group = rows_per_group;
+    p.ldr = ldr; p.ldo = ldo; p.out_dtype = out_dtype; p.act = act; p.form = form; p.limit = limit; p.alpha = alpha;
+    const long long row_bytes = (long long)p.k_groups * mx4::GROUP_BYTES;
+    CUtensorMap mw, mx;
+    if (int e = mx4_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, (long long)groups * rows_per_group, row_bytes, row_bytes, mx4::GROUP_BYTES, BM,
+                        CU_TENSOR_MAP_SWIZZLE_64B, "the codes")) return e;
+    if (int e = mx4_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, X, rows, K, (long long)ldx * 2, XK, tile, CU_TENSOR_MAP_SWIZZLE_128B, "the rows"))
+        return e;
+    cudaStream_t s = (cudaStream_t)stream;
+#define DD_MX4(T) \
+    case T: return dual ? launch_mx4<T, true>(mw, mx, p, s) : launch_mx4<T, false>(mw, mx, p, s);
+    switch (tile) {
+        DD_MX4(16)
+        DD_MX4(32)
+        DD_MX4(64)
+        DD_MX4(128)
+    }
+#undef DD_MX4
+    return dd_fail("dd_gemm_mx4: tile %d is not one of 16, 32, 64, 128", tile);
+}

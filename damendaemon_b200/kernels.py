@@ -115,6 +115,8 @@ _SIGNATURES = {
         "dd_gemm_tcgen05_plan": [_c_int, _c_int, _c_int, _c_int, _c_void, _c_void],
         "dd_gemm_grouped_tcgen05": [_c_void, _c_int, _c_void, _c_int, _c_int, _c_int, _c_void, _c_void, _c_int] + [_c_int] * 5
                                    + [_c_float, _c_float, _c_int, _c_void, _c_void, _c_int, _c_int, _c_void],
+        "dd_gemm_mx4": [_c_void, _c_int, _c_void, _c_void, _c_int, _c_int] + [_c_void] * 3 + [_c_int, _c_void, _c_void] + [_c_int] * 6
+                       + [_c_float, _c_float, _c_int, _c_int, _c_int, _c_void, _c_void],
         "dd_wait_probe": [ctypes.c_ulonglong, _c_void, _c_void, _c_void],
         "dd_attention_decode_supported": [_c_int] * 4,
         "dd_attention_prefill_supported": [_c_int] * 4,
@@ -1712,9 +1714,47 @@ def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, ou
     _here(a, w.codes, bias, residual, out)
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-    _call(library("core"), "dd_gemm_mx4_rows", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(),
-          _ptr(bias, "bias", torch.float32), _ptr(residual, "residual", torch.float32), 0 if residual is None else residual.stride(0),
-          _ptr(out, "out", out_dtype), out.stride(0), M, N, K, ACTIVATIONS[activation], kind, _stream())
+    bias, residual_stride = _ptr(bias, "bias", torch.float32), 0 if residual is None else residual.stride(0)
+    residual = _ptr(residual, "residual", torch.float32)
+    if M > MX4_FEW_ROWS and K % 8 == 0 and a.stride(0) % 8 == 0 and pointer % 16 == 0:
+        _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), 1, N, None, bias, residual,
+              residual_stride, None, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, 64 if M <= 64 else 128, 0, 0.0, 0.0, 0,
+              ACTIVATIONS[activation], kind, _ptr(error_flag(a.device)), _stream())
+    else:
+        _call(library("core"), "dd_gemm_mx4_rows", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), bias, residual,
+              residual_stride, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, ACTIVATIONS[activation], kind, _stream())
+    return out
+
+
+MX4_FEW_ROWS = 32        # up to here a product streams the matrix through mma.sync; beyond it goes to tcgen05 (rows of whole 16 bytes)
+
+
+def gemm_grouped_mx4(a, w, tile_group, tile, gated=None, out_dtype=None, activation=None, row_scale=None, out=None):
+    """gemm_grouped_tcgen05 with a stack of 4-bit matrices (w: an Mx4Matrix [groups, N, K], or [groups, 2 * inner, K] with
+    ``gated``): rows of a in tiles that meet one matrix each, with the gated unit or act(row_scale[r] * product) in the epilogue. The
+    rows of a tile whose group is negative are left as they are in ``out``."""
+    _rows(a, "a")
+    _check_row_scale(row_scale, a.shape[0])
+    if gated and (activation or row_scale is not None):
+        raise KernelError("grouped gemm: an activation or a row scale does not go with the gated unit")
+    if not isinstance(w, Mx4Matrix) or w.dim() != 3 or w.width != a.shape[1] or a.dtype != torch.bfloat16 or (gated and w.shape[1] % 2):
+        raise KernelError(f"grouped gemm: a {tuple(a.shape)} {a.dtype} does not fit the 4-bit matrices {tuple(w.shape)}")
+    rows, K = a.shape
+    groups, per_group = w.shape[0], w.shape[1]
+    N = per_group // 2 if gated else per_group
+    if tile not in GROUPED_TCGEN05_TILES or rows % tile or tile_group.numel() != rows // tile or not tile_group.is_contiguous():
+        raise KernelError(f"grouped gemm: {rows} rows in tiles of {tile} with {tile_group.numel()} groups")
+    _check_epilogue("grouped gemm", rows, N, None, None, out)
+    out_dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
+    kind, pointer = _dt(out_dtype), _ptr(a, "a")
+    _here(a, w.codes, tile_group, row_scale, out)
+    if out is None:
+        out = torch.empty((rows, N), dtype=out_dtype, device=a.device)
+    limit, alpha, form = (tuple(gated) + ("clamped_swish",))[:3] if gated else (0.0, 0.0, "clamped_swish")
+    _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), groups, per_group,
+          _ptr(tile_group, "tile_group", torch.int32), None, None, 0, _ptr(row_scale, "row_scale"), _ptr(out, "out", out_dtype), out.stride(0),
+          rows, N, K, int(tile), 1 if gated else 0, float(limit), float(alpha), GATED_FORMS[form], ACTIVATIONS[activation], kind,
+          _ptr(error_flag(a.device)), _stream())
     return out
 
 

@@ -185,3 +185,69 @@ def test_gemm_mx4_replayed():
             a.copy_(randn(seed, M, 320, dtype=torch.bfloat16))
             graph.replay()
             assert torch.equal(out, kernels.gemm_mx4(a, q))
+
+
+# ------------------------------------------------------------------ grouped products
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("N,K", [(1, 8), (100, 64), (128, 72), (130, 136), (257, 520), (64, 1600)])
+def test_grouped(tile, N, K):
+    groups = [2, 0, -1, 1, 1, 2, -1]
+    rows = tile * len(groups)
+    a, w = randn(N + K, rows, K, dtype=torch.bfloat16), randn(N + K + 1, 3, N, K, scale=K ** -0.5)
+    scale = randn(9, rows).abs()
+    q = kernels.mx4_quantize(w.to(DEV))
+    values = kernels.mx4_values(q, torch.float32).double().cpu()
+    tiles = torch.tensor(groups, dtype=torch.int32, device=DEV)
+    for act, row_scale, dtype in ((None, None, torch.bfloat16), (None, scale, torch.float32), ("relu2", scale, torch.float32), ("gelu", None, torch.bfloat16)):
+        out = torch.full((rows, N), 7.0, dtype=dtype, device=DEV)
+        got = kernels.gemm_grouped_mx4(a.to(DEV), q, tiles, tile, activation=act, out_dtype=dtype, out=out,
+                                       row_scale=None if row_scale is None else row_scale.to(DEV))
+        assert got is out
+        for i, e in enumerate(groups):
+            part = slice(i * tile, (i + 1) * tile)
+            if e < 0:
+                assert (got[part] == 7).all()
+                continue
+            by = 1.0 if row_scale is None else row_scale[part].double().unsqueeze(1)
+            z = a[part].double() @ values[e].t() * by
+            want = activation(z, act)
+            slope = 2 * z.abs() + 1 if act == "relu2" else 1.13
+            close(got[part], want, product_bound(a[part], values[e]) * by * slope + 2.0 ** -20 * (z.abs() + want.abs()))
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("inner,K", [(1, 8), (100, 64), (130, 200), (128, 520), (65, 1600)])
+@pytest.mark.parametrize("form", ["silu", "clamped_swish", "gelu_tanh"])
+def test_grouped_gated(tile, inner, K, form):
+    groups = [1, -1, 0, 1]
+    rows = tile * len(groups)
+    a, w = randn(inner + K, rows, K, dtype=torch.bfloat16), randn(inner + K + 1, 2, 2 * inner, K, scale=K ** -0.5)
+    q = kernels.mx4_quantize(w.to(DEV))
+    values = kernels.mx4_values(q, torch.float32).double().cpu()
+    tiles = torch.tensor(groups, dtype=torch.int32, device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        got = kernels.gemm_grouped_mx4(a.to(DEV), q, tiles, tile, gated=(2.0, 1.702, form), out_dtype=dtype)
+        for i, e in enumerate(groups):
+            if e < 0:
+                continue
+            part = slice(i * tile, (i + 1) * tile)
+            z, bound = a[part].double() @ values[e].t(), product_bound(a[part], values[e])
+            (gate, up), (bg, bu) = z.chunk(2, 1), bound.chunk(2, 1)
+            want = gated(gate, up, 2.0, 1.702, form)
+            # the unit's slopes: at most 1.13 (|up| + 1) by the gate, |gate| + 1 by up; its exponential is the special-function unit's, 2^-20
+            close(got[part], want, 1.13 * (up.abs() + 1) * bg + (gate.abs() + 1) * bu + 2.0 ** -18 * (want.abs() + gate.abs()))
+
+
+def test_grouped_refusals():
+    q = kernels.mx4_quantize(randn(1, 2, 32, 64).to(DEV))
+    a, tiles = torch.zeros(32, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    for bad in (lambda: kernels.gemm_grouped_mx4(a, q, tiles, 32), lambda: kernels.gemm_grouped_mx4(a, q, tiles, 8),
+                lambda: kernels.gemm_grouped_mx4(a[:, :60], q, tiles, 16), lambda: kernels.gemm_grouped_mx4(a.float(), q, tiles, 16),
+                lambda: kernels.gemm_grouped_mx4(a, q, tiles, 16, gated=(1.0, 1.0), activation="relu2"),
+                lambda: kernels.gemm_grouped_mx4(a, q, tiles.long(), 16), lambda: kernels.gemm_grouped_mx4(a, q, tiles, 16, out=a)):
+        with pytest.raises(kernels.KernelError):
+            bad()
+    odd = kernels.mx4_quantize(randn(1, 2, 32, 60).to(DEV))
+    with pytest.raises(kernels.KernelError, match="multiples of 8"):
+        kernels.gemm_grouped_mx4(a[:, :60], odd, tiles, 16)
