@@ -7,7 +7,7 @@
 ``run`` prints text deltas (token ids when the folder has no tokenizer) to standard output and
 the final usage/timing JSON to standard error. GPT-2 has no chat template, so ``--raw`` is the
 only prompt mode (docs/models.md:64-65 of the reference). Added here: --prompt-ids, --dtype,
---temperature, --top-p, --top-k, --seed, --ignore-eos, --page-size, --prefill-chunk-size.
+--feed-forward, --temperature, --top-p, --top-k, --seed, --ignore-eos, --page-size, --prefill-chunk-size.
 """
 from __future__ import annotations
 
@@ -31,6 +31,8 @@ def build_parser():
     run.add_argument("--no-graph", action="store_true", help="do not replay decode steps from CUDA graphs")
     run.add_argument("--device", choices=("cuda",), default="cuda")
     run.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16")
+    run.add_argument("--feed-forward", choices=("auto", "mx4"), default="auto",
+                     help="mx4: hold the feed-forwards' matrices in microscaled 4-bit numbers (bfloat16 only)")
     run.add_argument("--temperature", type=float, default=0)
     run.add_argument("--top-p", type=float, default=1)
     run.add_argument("--top-k", type=int, default=0)
@@ -61,7 +63,10 @@ def main(argv=None):
     if args.kv_cache_tokens is not None and args.kv_cache_tokens % args.page_size:
         print("error: --kv-cache-tokens must be a multiple of the page size", file=sys.stderr)
         return 2
-    runtime = Runtime(args.path, args.context, dtype=args.dtype, kv_cache_tokens=args.kv_cache_tokens, max_batch=1,
+    if args.feed_forward == "mx4" and args.dtype != "bfloat16":
+        print("error: --feed-forward mx4 goes with --dtype bfloat16", file=sys.stderr)
+        return 2
+    runtime = Runtime(args.path, args.context, dtype=args.dtype, feed_forward=args.feed_forward, kv_cache_tokens=args.kv_cache_tokens, max_batch=1,
                       page_size=args.page_size, use_graph=not args.no_graph, prefill_chunk_size=args.prefill_chunk_size)
     prompt = args.prompt if args.prompt is not None else [int(x) for x in args.prompt_ids.split(",") if x.strip()]
     for event in runtime.generate(prompt, args.max_tokens, ignore_eos=args.ignore_eos, temperature=args.temperature,

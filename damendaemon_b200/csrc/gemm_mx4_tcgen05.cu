@@ -153,11 +153,11 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const uint32_t* scales = p.scales + w_row * kgroups;
             constexpr int STEP = DUAL ? 1 : 2;
             const int first = DUAL ? 0 : set;
-            uint32_t four = first < kgroups ? __ldg(scales + first) : 0u;
+            uint32_t four = first < kgroups ? scales[first] : 0u;
             bool ok = true;
             for (int i = first; i < kgroups && ok; i += STEP) {
                 const uint32_t by = four;
-                if (i + STEP < kgroups) four = __ldg(scales + i + STEP);
+                if (i + STEP < kgroups) four = scales[i + STEP];
                 const int s = i % C::W_STAGES;
                 if (!tc::mbar_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
                 // a row is 64 bytes under the 64-byte swizzle: 16-byte piece t lies at t ^ (row / 2 % 4)
@@ -281,7 +281,7 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
                        int tile, int dual, float limit, float alpha, int form, int act, int out_dtype, int* error_flag, void* stream) {
     if (rows <= 0 || N <= 0) return 0;
     if (K <= 0 || K % 8 || ldx % 8) return dd_fail("dd_gemm_mx4: K=%d and the row stride %d must be multiples of 8 (TMA needs 16-byte rows)", K, ldx);
-    if (((uintptr_t)X & 15) || ((uintptr_t)codes & 15)) return dd_fail("dd_gemm_mx4: operands must be 16-byte aligned");
+    if (((uintptr_t)X & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3)) return dd_fail("dd_gemm_mx4: operands must be 16-byte aligned");
     if (out_dtype != DD_BF16 && out_dtype != DD_F32) return dd_fail("dd_gemm_mx4: unknown output dtype %d", out_dtype);
     if (tile <= 0 || (tile_group && rows % tile) || dd_ceil_div(rows, tile) > 65535) return dd_fail("dd_gemm_mx4: %d rows in tiles of %d", rows, tile);
     if (groups <= 0 || (groups > 1 && !tile_group) || rows_per_group != (dual ? 2 * N : N))

@@ -9,15 +9,20 @@
 // up_kernel: every cluster of blocks routes for itself (the router's rows are few and come from L2): its blocks share the router's
 // columns, send their partial logits to one another, and each block then chooses the tokens' experts, a warp a token, and
 // lists the distinct ones. The experts' gate and up rows are dealt out over the blocks of the whole grid, tiles of 8 + 8 rows (16 for plain
-// units); a block's warps share K. The unit's value, times the token's weight, is kept as float32 or as the sum of two bfloat16
-// numbers (16 bits: a hidden row rounded to one would be the layer's largest error by far).
-// down_kernel: a block owns 16 output rows and walks the chosen experts one after the other as one long sum; a token that does not use
-// an expert meets it with zeros. The blocks of a cluster share that sum. No atomics: a token's sums are added in a fixed order.
+// units). The unit's value, times the token's weight, is kept as float32 or as the sum of three bfloat16 numbers (24 bits, a float32's:
+// a hidden row rounded to one would be the layer's largest error by far, and two leave 2e-6 where float32 leaves 2e-7).
+// down_kernel: a block owns 16 output rows (float32: 4) and walks the chosen experts one after the other as one long sum, which its
+// warps share; a token that does not use an expert is passed over. No atomics: a token's sums are added in a fixed order.
 //
-// The streams are those of few_rows.cuh: weights straight into the registers of mma.sync (float32: multiply-adds).
+// Weights go to mma.sync (float32: to multiply-adds) through a ring of TMA boxes that every warp has for itself and that runs ahead
+// over the ends of its tiles: a warp waits for nobody but its own weights, and one lane asks for them (with cp.async, a lane's
+// address arithmetic for every 16 bytes kept the schedulers busy half of the time, and the streams at 4 TB/s). The shared unit's matrices
+// are asked into L2 while the tokens are being routed. mma.sync multiplies by eight columns: in up_kernel the tokens, in down_kernel
+// the terms of the tokens that use the expert, mostly one or two of them, so that one pass over them is enough.
 #include "few_rows.cuh"
 #include "route_choice.cuh"
 #include "tcgen05.cuh"
+#include <limits.h>
 
 // The layer's tensors and options, laid out as the Python side fills it (kernels.py: _ExpertLayer).
 struct DdExpertLayer {
@@ -35,7 +40,7 @@ struct DdExpertLayer {
 };
 
 namespace {
-constexpr int THREADS = 256, WARPS = 8, MAX_TOKENS = 8, MAX_TOP = 16, MAX_UNITS = MAX_TOKENS * MAX_TOP, MAX_OUTPUTS = 256;
+constexpr int UP_THREADS = 512, UP_WARPS = 16, TERMS = 3, SHARE_WIN = 12, MAX_TOKENS = 8, MAX_TOP = 16, MAX_UNITS = MAX_TOKENS * MAX_TOP, MAX_OUTPUTS = 256;
 enum Kind { F32 = 0, BF16 = 1, MX4 = 2 };
 
 // What up_kernel tells down_kernel.
@@ -53,51 +58,176 @@ struct Call {
     float* out;                  // [T, ldo]
     const int* ids;              // [T] (by table)
     Plan* plan;
-    uint8_t* hidden;             // [units][T][row], the shared unit's rows behind them
+    uint8_t* hidden;             // [units][T][terms][row], the shared unit's rows behind them
     int* error_flag;
     int T, ldy, ldr, ldo, max_units;
-    int row, shared_row;         // elements of a hidden row (two of them a token with bfloat16)
-    int w_wide, inner_wide, shared_wide, y_wide, cluster;
+    int row, shared_row;         // elements of a hidden row: whole steps, zeros behind the last feature
+    int y_wide, router_wide, w_wide, inner_wide;        // rows of whole 16-byte pieces (w: all matrices that meet y, inner: all down)
+    int cluster, y_pitch, stages;                                    // y_pitch: bytes of a token's row in up_kernel's shared memory
 };
+struct Maps { CUtensorMap gate_up, shared_gate_up, down, shared_down; };
 
 struct Tile { float sum[16][few::COLUMNS + 1]; };
+template <int N> struct Count { static constexpr int value = N; };
 
-// A warp's share (steps from .. to - 1) of 16 rows of a matrix [.., K] by all tokens, into dst.
-// row(i): the matrix row of the tile's row i. Kinds BF16 and MX4.
-template <bool FOUR_BITS, int TERMS, typename Row>
-__device__ __forceinline__ void tile_product(const void* w, const void* scales, int K, Row row, const __nv_bfloat16* x, const __nv_bfloat16* x2,
-                                             int from, int to, bool w_wide, bool x_wide, float* acc) {
+// What a warp multiplies at a time, a tile: 16 rows of a matrix on mma.sync, 4 with multiply-adds, as two boxes of half of them.
+template <int KIND> struct Stream {
+    static constexpr int ROWS = KIND == F32 ? few::F32_ROWS : 16, HALF = ROWS / 2;
+    static constexpr int STEP = KIND == BF16 ? 64 : 128;             // k
+    static constexpr int BOX_WIDTH = KIND == MX4 ? mx4::GROUP_BYTES : STEP, BOX_ROW = KIND == F32 ? 512 : KIND == BF16 ? 128 : 64;   // elements, bytes
+    static constexpr int BOX_BYTES = HALF * BOX_ROW, STAGE_BYTES = 2 * BOX_BYTES;
+    static constexpr int ELEMENT = KIND == F32 ? 4 : 2;
+    static constexpr int MOST_STAGES = 8192 / STAGE_BYTES;
+};
+__host__ __device__ constexpr int step_of(int kind) { return kind == BF16 ? 64 : 128; }
+
+// The boxes of a stage without TMA (rows that are no whole 16-byte pieces), in the layout that TMA gives them.
+template <int KIND>
+__device__ __forceinline__ void fill_stage(uint32_t slot, const void* matrix, size_t row_a, size_t row_b, size_t rows, int K, int step) {
+    using S = Stream<KIND>;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    for (int i = lane; i < S::STAGE_BYTES / 16; i += 32) {
+        const int r = i / (S::BOX_ROW / 16), piece = i % (S::BOX_ROW / 16);
+        const size_t row = min(r < S::HALF ? row_a + r : row_b + r - S::HALF, rows - 1);
+        if constexpr (KIND == F32) {
+            const float4 v = few::load4(reinterpret_cast<const float*>(matrix) + row * K, step * S::STEP + piece * 4, K, false);
+            few::sts16(slot + i * 16, make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)));
+        } else
+            few::sts16(slot + r * S::BOX_ROW + (piece ^ (r & 7)) * 16,
+                       few::load8(reinterpret_cast<const __nv_bfloat16*>(matrix) + row * K, step * S::STEP + piece * 8, K, false));
+    }
+    __syncwarp();
+}
+
+// A warp's ring. The fetching lane asks for stage after stage; every lane waits for them in the same order.
+template <int KIND> struct Ring {
+    using S = Stream<KIND>;
+    uint64_t* bars;
+    uint32_t base;
+    int stages, asked = 0, taken = 0;            // stage numbers; their phase follows from how often they wrapped
+    uint32_t phase = 0;
+    __device__ __forceinline__ Ring(uint64_t* b, uint32_t at, int n) : bars(b), base(at), stages(n) {}
+    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row_a, int row_b) {
+        uint64_t* bar = &bars[asked];
+        uint8_t* slot = reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES));
+        tc::mbar_expect_tx(bar, S::STAGE_BYTES);
+        tc::tma_load_2d(slot, map, step * S::BOX_WIDTH, row_a, bar);
+        tc::tma_load_2d(slot + S::BOX_BYTES, map, step * S::BOX_WIDTH, row_b, bar);
+    }
+    __device__ __forceinline__ void next_asked() { asked = asked + 1 == stages ? 0 : asked + 1; }
+    // the address of the next stage to read; `here`: it has been asked for
+    __device__ __forceinline__ uint32_t take(bool here, volatile int* gave_up) {
+        if (here) tc::mbar_wait(&bars[taken], phase, gave_up);
+        const uint32_t at = base + taken * S::STAGE_BYTES;
+        if (++taken == stages) { taken = 0; phase ^= 1; }
+        return at;
+    }
+};
+
+// 16-byte pieces of a step's other operand that a lane reads for one column, and where: on mma.sync lane (g, t) takes for row g
+// and g + 8 of the matrix the pieces 2 t and 2 t + 1 of 64 bfloat16 numbers (under TMA's 128-byte swizzle eight lanes then meet in
+// no bank), or the t-th eighth of every block of a 4-bit group.
+template <int KIND> constexpr int PIECES = KIND == MX4 ? 4 : 2;
+template <int KIND>
+__device__ __forceinline__ void take_column(uint4* b, const __nv_bfloat16* x, int step) {
+    const int t = threadIdx.x & 3;
+    const uint4* from = reinterpret_cast<const uint4*>(x + step * Stream<KIND>::STEP);
+#pragma unroll
+    for (int i = 0; i < PIECES<KIND>; ++i) b[i] = from[KIND == MX4 ? 4 * i + t : 2 * t + i];
+}
+// A step of a tile by P times eight columns. four0, four1: the scales of a 4-bit group of rows g and g + 8.
+template <int KIND, int P>
+__device__ __forceinline__ void mma_step(uint32_t slot, uint32_t four0, uint32_t four1, const uint4 (*b)[PIECES<KIND>], float (*d)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const size_t r0 = row(g), r1 = row(g + 8);
-    if (FOUR_BITS) {
-        const size_t groups = (K + mx4::GROUP - 1) / mx4::GROUP;
-        few::stream_mx4<TERMS>(reinterpret_cast<const uint4*>(w) + r0 * groups * 4 + t, reinterpret_cast<const uint4*>(w) + r1 * groups * 4 + t,
-                               reinterpret_cast<const uint32_t*>(scales) + r0 * groups, reinterpret_cast<const uint32_t*>(scales) + r1 * groups,
-                               x, x2, K, from, to, x_wide, acc);
+    if constexpr (KIND == MX4) {
+        const uint32_t at = slot + g * 64 + (t ^ (g >> 1 & 3)) * 16;
+        const uint4 a0 = few::lds16(at), a1 = few::lds16(at + Stream<KIND>::BOX_BYTES);
+        const uint32_t r0[4] = {a0.x, a0.y, a0.z, a0.w}, r1[4] = {a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t v0[4], v1[4];
+            mx4::pairs(r0[i], v0);
+            mx4::pairs(r1[i], v1);
+            const float by0 = mx4::scale(four0, i), by1 = mx4::scale(four1, i);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                float e[4] = {0.f, 0.f, 0.f, 0.f};
+                few::block_product(v0, v1, b[p][i], e);
+                few::add_block(by0, by1, e, d[p]);
+            }
+        }
     } else {
-        const __nv_bfloat16* m = reinterpret_cast<const __nv_bfloat16*>(w);
-        few::stream_bf16<TERMS>(m + r0 * K, m + r1 * K, x, x2, K, from, to, w_wide, x_wide, acc);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t at = slot + g * 128 + ((2 * t + i) ^ g) * 16;
+            const uint4 a0 = few::lds16(at), a1 = few::lds16(at + Stream<KIND>::BOX_BYTES);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                few::mma(d[p], a0.x, a1.x, a0.y, a1.y, b[p][i].x, b[p][i].y);
+                few::mma(d[p], a0.z, a1.z, a0.w, a1.w, b[p][i].z, b[p][i].w);
+            }
+        }
     }
 }
-__device__ __forceinline__ void put_tile(Tile& dst, const float* acc, float back) {
+template <int KIND>
+__device__ __forceinline__ void put_tile(Tile& to, const float* d) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dst.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = acc[i] * back;
+    for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i] * (KIND == MX4 ? few::MX4_BACK : 1.f);
 }
-// float32: four rows of the tile at a time, sums across the warp, into dst.
-template <int T>
-__device__ __forceinline__ void put_four(Tile& dst, int r0, float (*acc)[T]) {
-    float v[few::F32_ROWS * T];
+
+// Up to eight token numbers, ascending, four bits each.
+__device__ __forceinline__ uint32_t list_of(uint32_t users) {
+    uint32_t list = 0;
+    for (int shift = 0; users; users &= users - 1, shift += 4) list |= (uint32_t)(__ffs(users) - 1) << shift;
+    return list;
+}
+__device__ __forceinline__ int listed(uint32_t list, int i) { return list >> (4 * i) & 7; }
+
+// float32: a step of four rows by N tokens of a list; row t of the other operand: x + t * ld. Four tokens at a time: registers.
+template <int N>
+__device__ __forceinline__ void fma_step(uint32_t slot, const float* x, size_t ld, uint32_t list, int step, unsigned long long (*d)[N]) {
+    constexpr int H = N < 4 ? N : 4;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < N; h += H) {
+        float4 b[H];
+#pragma unroll
+        for (int i = 0; i < H; ++i) b[i] = *reinterpret_cast<const float4*>(x + listed(list, h + i) * ld + step * 128 + lane * 4);
+#pragma unroll
+        for (int r = 0; r < few::F32_ROWS; ++r) {
+            const uint4 v = few::lds16(slot + r * 512 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                few::fma_pair(d[r][h + i], __uint_as_float(v.x), __uint_as_float(v.y), b[i].x, b[i].y);
+                few::fma_pair(d[r][h + i], __uint_as_float(v.z), __uint_as_float(v.w), b[i].z, b[i].w);
+            }
+        }
+    }
+}
+// The warp's sums of rows r0 .. r0 + 3 and the first n tokens of a list, set or added in `to`.
+template <int N, bool ADD>
+__device__ __forceinline__ void put_rows(Tile& to, int r0, uint32_t list, int n, unsigned long long (*d)[N]) {
+    float v[few::F32_ROWS * N];
 #pragma unroll
     for (int r = 0; r < few::F32_ROWS; ++r)
 #pragma unroll
-        for (int t = 0; t < T; ++t) v[r * T + t] = acc[r][t];
-    const float sum = few::warp_sums<few::F32_ROWS * T>(v);
-    const int lane = threadIdx.x & 31, i = lane * (few::F32_ROWS * T) / 32;
-    if (lane % (32 / (few::F32_ROWS * T)) == 0) dst.sum[r0 + i / T][i % T] = sum;
+        for (int i = 0; i < N; ++i) v[r * N + i] = few::pair_sum(d[r][i]);
+    const float sum = few::warp_sums<few::F32_ROWS * N>(v);
+    const int lane = threadIdx.x & 31, at = lane * (few::F32_ROWS * N) / 32;
+    if (lane % (32 / (few::F32_ROWS * N)) == 0 && at % N < n) {
+        float& place = to.sum[r0 + at / N][listed(list, at % N)];
+        place = ADD ? place + sum : sum;
+    }
 }
-
-__device__ __forceinline__ int steps_of(int kind, int K) { return kind == BF16 ? (K + 31) / 32 : (K + 127) / 128; }
+// f(Count<N>) with N tokens at a time, N at least n.
+template <typename F> __device__ __forceinline__ void by_count(int n, F f) {
+    if (n == 1) f(Count<1>{});
+    else if (n == 2) f(Count<2>{});
+    else if (n <= 4) f(Count<4>{});
+    else f(Count<8>{});
+}
 
 // ---------------------------------------------------------------- routing, by every cluster for itself
 struct Routing {
@@ -105,79 +235,95 @@ struct Routing {
     float weight[MAX_TOKENS][MAX_TOP];
     float gate[MAX_TOKENS];                      // the shared unit's
     uint32_t users[MAX_OUTPUTS];                 // per output: which tokens chose it
-    int count[WARPS];
+    int count[UP_WARPS];
     int n_units;
     int expert[MAX_UNITS];
+    uint8_t unit_of[MAX_OUTPUTS];
+    float unit_weight[MAX_UNITS][MAX_TOKENS];    // a token's weight on a unit
+    uint64_t arrived;                            // the cluster's partial logits
 };
 
-// The logits of this block's share of the columns for all tokens, added over the warps that share them: part[row][token]
-template <int KIND, int T>
-__device__ void partial_logits(const Call& c, int rows, int from, int to, Tile* parts) {
-    const int warp = threadIdx.x >> 5;
-    const int tiles = (rows + 15) / 16, shares = max(1, WARPS / tiles), items = tiles * shares;
-    for (int item = warp; item < items; item += WARPS) {
-        const int tile = item % tiles, share = item / tiles;
-        const int a = from + (to - from) * share / shares, b = from + (to - from) * (share + 1) / shares;
-        auto row = [&](int i) { return (size_t)min(tile * 16 + i, rows - 1); };
+// Which rows and columns of the router a warp multiplies: items of 16 rows by a share of this block's columns.
+struct RouterItem {
+    int tile, from, to;
+    __device__ __forceinline__ RouterItem(const Call& c, int kind, int item) {
+        const int rows = c.l.experts + c.l.identity + c.l.shared_gate, tiles = (rows + 15) / 16, shares = max(1, UP_WARPS / tiles);
+        const int steps = (c.l.width + (kind == F32 ? 127 : 31)) / (kind == F32 ? 128 : 32), rank = c.cluster > 1 ? (int)tc::cluster_rank() : 0;
+        const int begin = steps * rank / c.cluster, end = steps * (rank + 1) / c.cluster, share = item / tiles;
+        tile = item % tiles;
+        from = begin + (end - begin) * share / shares;
+        to = begin + (end - begin) * (share + 1) / shares;
+    }
+};
+__device__ __forceinline__ const __nv_bfloat16* router_row(const Call& c, int tile, int i) {
+    return reinterpret_cast<const __nv_bfloat16*>(c.l.router) +
+           (size_t)min(tile * 16 + i, c.l.experts + c.l.identity + c.l.shared_gate - 1) * c.l.router_stride;
+}
+
+// The logits of the block's columns for all tokens, by item. ahead: the first item's first steps.
+template <int KIND>
+__device__ void partial_logits(const Call& c, const uint8_t* y, int items, Tile* parts, few::Ahead& ahead) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    for (int item = warp; item < items; item += UP_WARPS) {
+        const RouterItem it(c, KIND, item);
         if constexpr (KIND == F32) {
-            const float* m = reinterpret_cast<const float*>(c.l.router);
+            const int last = c.l.experts + c.l.identity + c.l.shared_gate - 1;
             for (int r0 = 0; r0 < 16; r0 += few::F32_ROWS) {
                 const float* w[few::F32_ROWS];
-                float acc[few::F32_ROWS][T];
+                unsigned long long acc[few::F32_ROWS][MAX_TOKENS] = {};
 #pragma unroll
-                for (int r = 0; r < few::F32_ROWS; ++r) {
-                    w[r] = m + row(r0 + r) * c.l.router_stride;
-#pragma unroll
-                    for (int t = 0; t < T; ++t) acc[r][t] = 0.f;
-                }
-                few::stream_f32<T>(w, reinterpret_cast<const float*>(c.y), c.ldy, (1u << c.T) - 1, c.l.width, a, b, c.w_wide, c.y_wide, acc);
-                put_four<T>(parts[item], r0, acc);
+                for (int r = 0; r < few::F32_ROWS; ++r)
+                    w[r] = reinterpret_cast<const float*>(c.l.router) + (size_t)min(it.tile * 16 + r0 + r, last) * c.l.router_stride;
+                few::stream_f32<MAX_TOKENS>(w, reinterpret_cast<const float*>(y), c.y_pitch / 4, (1u << c.T) - 1, c.l.width, it.from, it.to, c.router_wide,
+                                            true, acc);
+                put_rows<MAX_TOKENS, false>(parts[item], r0, 0x76543210u, MAX_TOKENS, acc);
             }
         } else {
-            const int lane = threadIdx.x & 31, g = lane >> 2;
-            const __nv_bfloat16* m = reinterpret_cast<const __nv_bfloat16*>(c.l.router);
-            const __nv_bfloat16* x = g < c.T ? reinterpret_cast<const __nv_bfloat16*>(c.y) + (size_t)g * c.ldy : nullptr;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            few::stream_bf16<1>(m + row(g) * c.l.router_stride, m + row(g + 8) * c.l.router_stride, x, nullptr, c.l.width, a, b, c.w_wide,
-                                c.y_wide, acc);
-            put_tile(parts[item], acc, 1.f);
+            const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(y + min(g, c.T - 1) * c.y_pitch);
+            const __nv_bfloat16 *w0 = router_row(c, it.tile, g), *w1 = router_row(c, it.tile, g + 8);
+            if (item != warp) ahead.load(w0, w1, c.l.width, it.from, it.to, c.router_wide);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            few::stream_bf16(w0, w1, x, c.l.width, it.from, it.to, c.router_wide, ahead, d);
+            put_tile<BF16>(parts[item], d);
         }
     }
 }
 
-template <int KIND, int T>
-__device__ void route(const Call& c, Routing& r, float* scratch) {
+template <int KIND>
+__device__ void route(const Call& c, const uint8_t* y, Routing& r, float* scratch, few::Ahead& ahead, volatile int* gave_up) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int outputs = c.l.experts + c.l.identity;
-    for (int e = threadIdx.x; e < MAX_OUTPUTS; e += THREADS) r.users[e] = 0;
+    if (threadIdx.x < MAX_OUTPUTS) r.users[threadIdx.x] = 0;
     if (c.l.router) {
-        const int rows = outputs + c.l.shared_gate, tiles = (rows + 15) / 16, shares = max(1, WARPS / tiles);
+        const int rows = outputs + c.l.shared_gate, tiles = (rows + 15) / 16, shares = max(1, UP_WARPS / tiles);
         const int n = tiles * 16 * MAX_TOKENS;                          // logits, a row of eight an output
         const int rank = c.cluster > 1 ? (int)tc::cluster_rank() : 0;
         Tile* parts = reinterpret_cast<Tile*>(scratch);
         float* sums = scratch + (sizeof(Tile) / 4) * tiles * shares;     // [cluster][n]: what every block of the cluster found
-        const int steps = steps_of(KIND == F32 ? F32 : BF16, c.l.width);
-        partial_logits<KIND, T>(c, rows, steps * rank / c.cluster, steps * (rank + 1) / c.cluster, parts);
+        partial_logits<KIND>(c, y, tiles * shares, parts, ahead);
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += THREADS) {
+        for (int i = threadIdx.x; i < n; i += UP_THREADS) {
             const int row = i / MAX_TOKENS, t = i % MAX_TOKENS;
             float z = 0.f;
             if (t < c.T)
+#pragma unroll 1
                 for (int s = 0; s < shares; ++s) z += parts[s * tiles + row / 16].sum[row % 16][t];
             if (c.cluster == 1) sums[i] = z;
             else
-                for (int to = 0; to < c.cluster; ++to) tc::st_cluster_f32(tc::map_to_rank(&sums[rank * n + i], to), z);
+#pragma unroll 1
+                for (int to = 0; to < c.cluster; ++to) tc::st_async_f32(tc::map_to_rank(&sums[rank * n + i], to), z, tc::map_to_rank(&r.arrived, to));
         }
         if (c.cluster > 1) {
-            tc::cluster_arrive();
-            tc::cluster_wait();
+            if (threadIdx.x == 0) tc::mbar_expect_tx(&r.arrived, c.cluster * n * 4);
+            tc::mbar_wait(&r.arrived, 0, gave_up);
         } else __syncthreads();
         float* value = sums + c.cluster * n;                            // [T][outputs]
         float* score = value + MAX_TOKENS * outputs;
         float* worth = score + MAX_TOKENS * outputs;
-        for (int i = threadIdx.x; i < rows * MAX_TOKENS; i += THREADS) {
+        for (int i = threadIdx.x; i < rows * MAX_TOKENS; i += UP_THREADS) {
             const int e = i / MAX_TOKENS, t = i % MAX_TOKENS;
             float z = 0.f;
+#pragma unroll 1
             for (int s = 0; s < c.cluster; ++s) z += sums[s * n + i];
             if (e >= outputs) r.gate[t] = 1.0f / (1.0f + expf(-z));
             else if (c.l.softmax) value[t * outputs + e] = z;
@@ -185,22 +331,30 @@ __device__ void route(const Call& c, Routing& r, float* scratch) {
         }
         if (!c.l.shared_gate && threadIdx.x < MAX_TOKENS) r.gate[threadIdx.x] = 1.f;
         __syncthreads();
-        if (warp < c.T)
-            dd_choose_experts(score + warp * outputs, value + warp * outputs, worth + warp * c.l.groups, outputs, c.l.top, c.l.groups, c.l.keep,
-                              c.l.weight_scale, c.l.softmax, c.l.correction, c.l.renormalize, r.chosen[warp], r.weight[warp]);
+        if (warp < c.T) {
+            float *sc = score + warp * outputs, *v = value + warp * outputs, *wo = worth + warp * max(c.l.groups, MAX_TOP);
+            if (outputs <= 64)
+                dd_choose_few<2>(sc, v, wo, outputs, c.l.top, c.l.groups, c.l.keep, c.l.weight_scale, c.l.softmax, c.l.correction, c.l.renormalize,
+                                 r.chosen[warp], r.weight[warp]);
+            else
+                dd_choose_few<MAX_OUTPUTS / 32>(sc, v, wo, outputs, c.l.top, c.l.groups, c.l.keep, c.l.weight_scale, c.l.softmax, c.l.correction,
+                                                c.l.renormalize, r.chosen[warp], r.weight[warp]);
+        }
     } else {
-        for (int i = threadIdx.x; i < c.T * c.l.top; i += THREADS) {
-            const int t = i / c.l.top, k = i % c.l.top, id = c.ids[t];
-            const int e = id >= 0 && id < c.l.vocab ? c.l.table[(size_t)id * c.l.top + k] : -1;
-            r.chosen[t][k] = e;
+        const int t = threadIdx.x / MAX_TOP, k = threadIdx.x % MAX_TOP;
+        if (t < c.T && k < c.l.top) {
+            const int id = c.ids[t];
+            r.chosen[t][k] = id >= 0 && id < c.l.vocab ? c.l.table[(size_t)id * c.l.top + k] : -1;
             r.weight[t][k] = c.l.weight_scale;
         }
         if (threadIdx.x < MAX_TOKENS) r.gate[threadIdx.x] = 1.f;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < c.T * c.l.top; i += THREADS) {
-        const int t = i / c.l.top, e = r.chosen[t][i % c.l.top];
-        if (e >= 0 && e < outputs) atomicOr(&r.users[e], 1u << t);
+    const int pair_t = threadIdx.x / MAX_TOP, pair_k = threadIdx.x % MAX_TOP;        // a thread a (token, choice)
+    const bool pair = pair_t < c.T && pair_k < c.l.top;
+    const int pair_e = pair ? r.chosen[pair_t][pair_k] : -1;
+    if (pair) {
+        if (pair_e >= 0 && pair_e < outputs) atomicOr(&r.users[pair_e], 1u << pair_t);
         else if (blockIdx.x == 0) atomicOr(c.error_flag, 1);           // an expert out of range: left out, and reported
     }
     __syncthreads();
@@ -209,263 +363,542 @@ __device__ void route(const Call& c, Routing& r, float* scratch) {
     const uint32_t votes = __ballot_sync(0xffffffffu, used);
     if (lane == 0) r.count[warp] = __popc(votes);
     __syncthreads();
-    int at = __popc(votes & ((1u << lane) - 1));
-    for (int w = 0; w < warp; ++w) at += r.count[w];
-    if (used) r.expert[at] = threadIdx.x;
-    if (threadIdx.x == 0) {
-        int total = 0;
-        for (int w = 0; w < WARPS; ++w) total += r.count[w];
-        r.n_units = total;
+    int at = __popc(votes & ((1u << lane) - 1)), total = 0;
+#pragma unroll 1
+    for (int w = 0; w < MAX_OUTPUTS / 32; ++w) {
+        if (w < warp) at += r.count[w];
+        total += r.count[w];
+    }
+    if (used) {
+        r.expert[at] = threadIdx.x;
+        r.unit_of[threadIdx.x] = (uint8_t)at;
+    }
+    if (threadIdx.x == 0) r.n_units = total;
+    __syncthreads();
+    if (pair_e >= 0 && pair_e < c.l.experts) {    // a token's choices of an expert (a table may name one twice), by the first of them
+        float w = 0.f;
+        bool first = true;
+#pragma unroll 1
+        for (int i = 0; i < c.l.top; ++i)
+            if (r.chosen[pair_t][i] == pair_e) {
+                w += r.weight[pair_t][i];
+                if (i < pair_k) first = false;
+            }
+        if (first) r.unit_weight[r.unit_of[pair_e]][pair_t] = w;
     }
     __syncthreads();
 }
-// A token's weight on an expert: its choices of it (a table may name one twice), in their order.
-__device__ __forceinline__ float weight_of(const Call& c, const Routing& r, int t, int e) {
-    float w = 0.f;
-    for (int k = 0; k < c.l.top; ++k)
-        if (r.chosen[t][k] == e) w += r.weight[t][k];
-    return w;
+
+// Asks for a matrix in L2, shared out over the grid's threads (4 KB each time).
+__device__ __forceinline__ void ask_for(const void* base, size_t bytes) {
+    constexpr size_t PIECE = 4096;
+    const size_t n = bytes / PIECE, threads = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = (size_t)threadIdx.x * gridDim.x + blockIdx.x; i < n; i += threads)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<const uint8_t*>(base) + i * PIECE), "r"((uint32_t)PIECE) : "memory");
+}
+__device__ __forceinline__ size_t matrix_bytes(int kind, size_t rows, int K) {
+    return kind == MX4 ? rows * ((K + mx4::GROUP - 1) / mx4::GROUP) * mx4::GROUP_BYTES : rows * K * (kind == F32 ? 4 : 2);
 }
 
-template <int KIND, int T>
-__global__ void __launch_bounds__(THREADS, 2)
-up_kernel(const __grid_constant__ Call c) {
-    extern __shared__ __align__(16) float scratch[];
+// The barriers of a block's rings, and whether one of its waits ran out.
+template <int W> struct Barriers {
+    uint64_t full[W][8];
+    int gave_up;
+    __device__ __forceinline__ void init() {
+        for (int i = threadIdx.x; i < W * 8; i += W * 32) tc::mbar_init(&full[i / 8][i % 8], 1);
+        if (threadIdx.x == 0) gave_up = 0;
+        tc::fence_barrier_init();
+        tc::fence_proxy_async();
+    }
+};
+// A unit's value, in float32, as its hidden row keeps it.
+template <int KIND>
+__device__ __forceinline__ void put_hidden(const Call& c, bool shared, int unit, int t, int feature, float v) {
+    const int row = shared ? c.shared_row : c.row;
+    const size_t slot = shared ? (size_t)t : (size_t)unit * c.T + t, before = shared ? (size_t)c.max_units * c.T * c.row : 0;
+    if constexpr (KIND == F32) reinterpret_cast<float*>(c.hidden)[before + slot * row + feature] = v;
+    else {
+        __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(c.hidden) + before * TERMS + slot * TERMS * row + feature;
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) {
+            const __nv_bfloat16 term = __float2bfloat16_rn(v);
+            h[i * row] = term;
+            v -= __bfloat162float(term);
+        }
+    }
+}
+// (Not inlined: the kernel is read from L2 once for every launch, and its instructions are what a small layer waits for.)
+__device__ __noinline__ float unit_value(const Call& c, bool shared, float a, float b, float by) {
+    if (shared) return by * dd_gated_value<false>(a, b, c.l.shared_form, c.l.shared_limit, c.l.shared_alpha);
+    if (c.l.gated) return by * dd_gated_value<false>(a, b, c.l.form, c.l.limit, c.l.alpha);
+    return c.l.weight_input ? dd_activation(by * a, c.l.act) : by * dd_activation(a, c.l.act);
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(UP_THREADS, 1)
+up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
+    using S = Stream<KIND>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Routing r;
-    __shared__ Tile red[2][WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ Tile red[2][UP_WARPS];
+    __shared__ Barriers<UP_WARPS> bars;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, width = c.l.width;
     dd_launch_dependents();
-    if (c.cluster > 1) {                          // a block's shared memory may be written once it runs
+    if (c.l.shared_inner && c.w_wide) ask_for(c.l.shared_gate_up, matrix_bytes(KIND, (size_t)2 * c.l.shared_inner, width));
+    few::Ahead ahead;                             // of the router, also a weight
+    if (KIND != F32 && c.l.router) {
+        const RouterItem it(c, KIND, warp);
+        if (it.from < it.to) ahead.load(router_row(c, it.tile, lane >> 2), router_row(c, it.tile, (lane >> 2) + 8), width, it.from, it.to, c.router_wide);
+    }
+    bars.init();
+    if (threadIdx.x == 0) {
+        tc::mbar_init(&r.arrived, 1);
+        tc::fence_barrier_init();
+    }
+    if (c.cluster > 1) {                          // a block's shared memory may be written once it runs and has its barrier
         tc::cluster_arrive();
         tc::cluster_wait();
     }
     dd_grid_wait();
-    route<KIND, T>(c, r, scratch);
+    // the tokens' rows with zeros behind them; a row starts 16 bytes off the one before it, modulo 128, so that eight lanes' pieces
+    // of two rows meet in no bank
+    uint8_t* y = smem + UP_WARPS * c.stages * S::STAGE_BYTES;
+    {
+        const int pieces = (c.y_pitch - 16) / 16, in = 16 / S::ELEMENT;
+        const int by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;          // warps a token
+        if (t < c.T)
+#pragma unroll 1
+            for (int at = (warp % by) * 32 + lane; at < pieces; at += by * 32) {
+                uint4 v;
+                if constexpr (KIND == F32) {
+                    const float4 f = few::load4(reinterpret_cast<const float*>(c.y) + (size_t)t * c.ldy, at * in, width, c.y_wide);
+                    v = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w));
+                } else v = few::load8(reinterpret_cast<const __nv_bfloat16*>(c.y) + (size_t)t * c.ldy, at * in, width, c.y_wide);
+                *reinterpret_cast<uint4*>(y + t * c.y_pitch + at * 16) = v;
+            }
+    }
+    __syncthreads();
+    route<KIND>(c, y, r, reinterpret_cast<float*>(y + c.T * c.y_pitch), ahead, &bars.gave_up);
     if (blockIdx.x == 0) {
-        for (int u = threadIdx.x; u < r.n_units; u += THREADS) {
+        for (int u = threadIdx.x; u < r.n_units; u += UP_THREADS) {
             c.plan->expert[u] = r.expert[u];
             c.plan->tokens[u] = r.users[r.expert[u]];
         }
         if (threadIdx.x == 0) c.plan->n_units = r.n_units;
         if (threadIdx.x < c.T) {
             float own = 0.f;
+#pragma unroll 1
             for (int k = 0; k < c.l.top; ++k)
                 if (r.chosen[threadIdx.x][k] >= c.l.experts && r.chosen[threadIdx.x][k] < c.l.experts + c.l.identity) own += r.weight[threadIdx.x][k];
             c.plan->own[threadIdx.x] = own;
         }
     }
-    const int tile_rows = c.l.gated ? 8 : 16;
-    const int per_unit = (c.l.inner + tile_rows - 1) / tile_rows, for_shared = (c.l.shared_inner + 7) / 8;
-    const int total = r.n_units * per_unit + for_shared;
-    const int steps = steps_of(KIND, c.l.width);
-    int turn = 0;
-    for (int task = blockIdx.x; task < total; task += gridDim.x, turn ^= 1) {
-        const int unit = task < r.n_units * per_unit ? task / per_unit : -1;         // -1: the shared one
-        const int tile = unit >= 0 ? task % per_unit : task - r.n_units * per_unit;
-        const int inner = unit >= 0 ? c.l.inner : c.l.shared_inner;
-        const bool gated = unit < 0 || c.l.gated;
-        const size_t base = unit >= 0 ? (size_t)r.expert[unit] * inner * (gated ? 2 : 1) : 0;
-        const int first = tile * (gated ? 8 : 16);
-        // rows 0..7 are gate rows and 8..15 the same features' up rows; plain: sixteen neighbours
-        auto row = [&](int i) { return gated ? base + (i < 8 ? 0 : inner) + min(first + (i & 7), inner - 1) : base + min(first + i, inner - 1); };
-        const void* w = unit >= 0 ? c.l.gate_up : c.l.shared_gate_up;
-        const void* scales = unit >= 0 ? c.l.gate_up_scales : c.l.shared_gate_up_scales;
-        const int from = steps * warp / WARPS, to = steps * (warp + 1) / WARPS;
-        Tile* parts = red[turn];
-        if constexpr (KIND == F32) {
-            for (int r0 = 0; r0 < 16; r0 += few::F32_ROWS) {
-                const float* rows[few::F32_ROWS];
-                float acc[few::F32_ROWS][T];
-#pragma unroll
-                for (int i = 0; i < few::F32_ROWS; ++i) {
-                    rows[i] = reinterpret_cast<const float*>(w) + row(r0 + i) * c.l.width;
-#pragma unroll
-                    for (int t = 0; t < T; ++t) acc[i][t] = 0.f;
-                }
-                few::stream_f32<T>(rows, reinterpret_cast<const float*>(c.y), c.ldy, (1u << c.T) - 1, c.l.width, from, to, c.w_wide, c.y_wide, acc);
-                put_four<T>(parts[warp], r0, acc);
-            }
-        } else {
-            const int g = lane >> 2;
-            const __nv_bfloat16* x = g < c.T ? reinterpret_cast<const __nv_bfloat16*>(c.y) + (size_t)g * c.ldy : nullptr;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            tile_product<KIND == MX4, 1>(w, scales, c.l.width, row, x, nullptr, from, to, c.w_wide, c.y_wide, acc);
-            put_tile(parts[warp], acc, KIND == MX4 ? few::MX4_BACK : 1.f);
-        }
-        __syncthreads();          // (the other set of tiles is written next: one barrier a task is enough)
-        const int rows = gated ? 8 : 16;
-        for (int i = threadIdx.x; i < rows * MAX_TOKENS; i += THREADS) {
-            const int t = i / rows, f = i % rows, feature = first + f;
-            const int hidden_row = unit >= 0 ? c.row : c.shared_row;
-            if (t >= c.T || feature >= hidden_row || (unit >= 0 && !(r.users[r.expert[unit]] >> t & 1))) continue;
-            float v = 0.f;                        // (zeros between the last feature and the end of the row)
-            if (feature < inner) {
-                float a = 0.f, b = 0.f;
-#pragma unroll
-                for (int s = 0; s < WARPS; ++s) a += parts[s].sum[f][t];
-                if (gated)
-#pragma unroll
-                    for (int s = 0; s < WARPS; ++s) b += parts[s].sum[f + 8][t];
-                const float by = unit >= 0 ? weight_of(c, r, t, r.expert[unit]) : r.gate[t];
-                if (unit < 0) v = by * dd_gated_value<false>(a, b, c.l.shared_form, c.l.shared_limit, c.l.shared_alpha);
-                else if (gated) v = by * dd_gated_value<false>(a, b, c.l.form, c.l.limit, c.l.alpha);
-                else v = c.l.weight_input ? dd_activation(by * a, c.l.act) : by * dd_activation(a, c.l.act);
-            }
-            const size_t slot = unit >= 0 ? (size_t)unit * c.T + t : (size_t)t;
-            if constexpr (KIND == F32) {
-                float* h = reinterpret_cast<float*>(c.hidden) + (unit >= 0 ? 0 : (size_t)c.max_units * c.T * c.row);
-                h[slot * hidden_row + feature] = v;
-            } else {
-                __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(c.hidden) + (unit >= 0 ? 0 : (size_t)c.max_units * c.T * c.row * 2);
-                const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-                h[slot * 2 * hidden_row + feature] = hi;
-                h[(slot * 2 + 1) * hidden_row + feature] = __float2bfloat16_rn(v - __bfloat162float(hi));
-            }
-        }
+    // tiles: the shared unit's, then every chosen expert's
+    const int features = c.l.gated ? S::HALF : S::ROWS;
+    const int per_unit = (c.l.inner + features - 1) / features, for_shared = (c.l.shared_inner + S::HALF - 1) / S::HALF;
+    const int total = for_shared + r.n_units * per_unit;
+    // `share` warps share a tile's columns: what leaves the fewest warps idle in the last round (the tiles are dealt out over the
+    // blocks first). A tile alone in a warp needs no barrier of the block, so sharers have to win a quarter of the time.
+    const int warps = gridDim.x * UP_WARPS;
+    int share = 1;
+#pragma unroll 1
+    for (int s = 2, best = (total + warps - 1) / warps * 16; s <= UP_WARPS; s *= 2) {
+        const int cost = (total * s + warps - 1) / warps * 16 / s;
+        if (cost < best * SHARE_WIN / 16) { best = cost; share = s; }
     }
-}
-
-template <int KIND, int T>
-__global__ void __launch_bounds__(THREADS, 2)
-down_kernel(const __grid_constant__ Call c) {
-    __shared__ Tile red[WARPS];
-    __shared__ float others[7][16][MAX_TOKENS];          // the sums of the cluster's other blocks
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cluster = c.cluster, rank = cluster > 1 ? (int)tc::cluster_rank() : 0;
-    dd_launch_dependents();
-    if (cluster > 1) {
-        tc::cluster_arrive();
-        tc::cluster_wait();
-    }
-    dd_grid_wait();
-    const int n0 = blockIdx.x / cluster * 16;
-    const int n_units = c.plan->n_units;
-    const int per_unit = steps_of(KIND, c.l.inner), for_shared = c.l.shared_inner ? steps_of(KIND, c.l.shared_inner) : 0;
-    const int total = n_units * per_unit + for_shared;
-    const int index = rank * WARPS + warp, sharers = cluster * WARPS;
-    const int from = (int)((long long)total * index / sharers), to = (int)((long long)total * (index + 1) / sharers);
-    auto each_run = [&](auto run) {              // the runs of steps of one unit in this warp's share
-        for (int at = from; at < to;) {
-            const int unit = at < n_units * per_unit ? at / per_unit : n_units;
-            const int begin = unit * per_unit, end = min(to, unit < n_units ? begin + per_unit : total);
-            run(unit, at - begin, end - begin);
-            at = end;
+    const int slots = UP_WARPS / share, slot = warp / share, part = warp % share, stride = gridDim.x * slots;
+    const int steps = (width + S::STEP - 1) / S::STEP, from = steps * part / share, to = steps * (part + 1) / share;
+    // a tile: its unit (-1: the shared one), first feature, and the rows of the matrix where its two boxes begin: gate rows and the same
+    // features' up rows; plain: neighbours
+    struct Place { int unit, first, row_a, row_b; };
+    auto place_of = [&](int tile) {
+        Place p;
+        p.unit = tile < for_shared ? -1 : (tile - for_shared) / per_unit;
+        const bool gated = p.unit < 0 || c.l.gated;
+        const int inner = p.unit < 0 ? c.l.shared_inner : c.l.inner;
+        p.first = p.unit < 0 ? tile * S::HALF : (tile - for_shared - p.unit * per_unit) * features;
+        p.row_a = (p.unit < 0 ? 0 : r.expert[p.unit] * inner * (gated ? 2 : 1)) + p.first;
+        p.row_b = p.row_a + (gated ? inner : S::HALF);
+        return p;
+    };
+    Ring<KIND> ring(bars.full[warp], tc::smem_u32(smem) + warp * c.stages * S::STAGE_BYTES, c.stages);
+    // the ring's fetching end
+    int f_tile = slot * gridDim.x + blockIdx.x, f_step = from;
+    Place f = {};
+    if (f_tile < total) f = place_of(f_tile);
+    auto fetch = [&] {
+        if (f_tile >= total || from >= to) return;
+        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.row_a, f.row_b);
+        ring.next_asked();
+        if (++f_step == to) {
+            f_step = from;
+            f_tile += stride;
+            if (f_tile < total) f = place_of(f_tile);
         }
     };
-    if constexpr (KIND == F32) {
-        for (int r0 = 0; r0 < 16; r0 += few::F32_ROWS) {
-            float acc[few::F32_ROWS][T];
+#pragma unroll 1
+    for (int i = 0; i < c.stages - 1; ++i) fetch();
+    // (columns beyond the tokens read the last one's row; nobody looks at them)
+    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(y + min(lane >> 2, c.T - 1) * c.y_pitch);
+    // (with shared tiles every warp of the block takes part in every round's barrier)
+    for (int turn = 0, round = blockIdx.x; round < total; round += stride, turn ^= 1) {
+        const int tile = round + slot * gridDim.x;
+        const bool mine = tile < total;
+        const Place p = place_of(mine ? tile : 0);
+        const bool shared = p.unit < 0;
+        const uint32_t users = shared ? (1u << c.T) - 1 : r.users[r.expert[p.unit]];
+        const void* matrix = shared ? c.l.shared_gate_up : c.l.gate_up;
+        const size_t matrix_rows = shared ? (size_t)2 * c.l.shared_inner : (size_t)c.l.experts * c.l.inner * (c.l.gated ? 2 : 1);
+        auto next = [&](int s) {
+            const uint32_t at = ring.take(c.w_wide, &bars.gave_up);
+            if (!c.w_wide) fill_stage<KIND>(at, matrix, p.row_a, p.row_b, matrix_rows, width, s);
+            return at;
+        };
+        if constexpr (KIND == F32) {
+            if (mine)
+                by_count(__popc(users), [&](auto count) {
+                    constexpr int N = decltype(count)::value;
+                    const uint32_t list = list_of(users);         // (what it lacks to N names token 0 again, and is dropped)
+                    unsigned long long d[few::F32_ROWS][N] = {};
+                    for (int s = from; s < to; ++s) {
+                        fma_step<N>(next(s), reinterpret_cast<const float*>(y), c.y_pitch / 4, list, s, d);
+                        __syncwarp();
+                        fetch();          // into the stage before this one, which the warp has read
+                    }
+                    put_rows<N, false>(red[turn][warp], 0, list, __popc(users), d);
+                });
+            if (share > 1) __syncthreads();          // (the other set is written next: one barrier a round is enough)
+            else __syncwarp();
+            if (mine && part == 0) {
+                const int n = shared || c.l.gated ? S::HALF : S::ROWS;
+                for (int i = lane; i < n * c.T; i += 32) {
+                    const int t = i / n, k = i % n, feature = p.first + k;
+                    if (feature >= (shared ? c.l.shared_inner : c.l.inner) || !(users >> t & 1)) continue;
+                    float a = 0.f, b = 0.f;
+                    for (int s = 0; s < share; ++s) {
+                        const Tile& have = red[turn][slot * share + s];
+                        a += have.sum[k][t];
+                        if (n == S::HALF) b += have.sum[k + S::HALF][t];
+                    }
+                    put_hidden<KIND>(c, shared, p.unit, t, feature, unit_value(c, shared, a, b, shared ? r.gate[t] : r.unit_weight[p.unit][t]));
+                }
+            }
+        } else {
+            float d[1][4] = {};
+            if (mine) {
+                const uint32_t *s0 = nullptr, *s1 = nullptr;
+                uint32_t four0 = 0, four1 = 0;
+                if (KIND == MX4) {
+                    const size_t groups = steps, last = matrix_rows - 1;
+                    const uint32_t* scales = reinterpret_cast<const uint32_t*>(shared ? c.l.shared_gate_up_scales : c.l.gate_up_scales);
+                    s0 = scales + min((size_t)p.row_a + (lane >> 2), last) * groups;
+                    s1 = scales + min((size_t)p.row_b + (lane >> 2), last) * groups;
+                    if (from < to) { four0 = s0[from]; four1 = s1[from]; }
+                }
+                for (int s = from; s < to; ++s) {
+                    uint4 b[1][PIECES<KIND>];
+                    take_column<KIND>(b[0], x, s);
+                    uint32_t n0 = 0, n1 = 0;
+                    if (KIND == MX4 && s + 1 < to) { n0 = s0[s + 1]; n1 = s1[s + 1]; }
+                    mma_step<KIND, 1>(next(s), four0, four1, b, d);
+                    four0 = n0; four1 = n1;
+                    __syncwarp();
+                    fetch();
+                }
+            }
+            if (share > 1) {                      // the first of the sharers adds up
+                put_tile<KIND>(red[turn][warp], d[0]);
+                __syncthreads();
+                if (mine && part == 0) {
+                    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-            for (int i = 0; i < few::F32_ROWS; ++i)
+                    for (int i = 0; i < 4; ++i) {
+                        float sum = 0.f;
+                        for (int s = 0; s < share; ++s) sum += red[turn][warp + s].sum[g + 8 * (i >> 1)][2 * t + (i & 1)];
+                        d[0][i] = sum;
+                    }
+                }
+            } else if (KIND == MX4)
 #pragma unroll
-                for (int t = 0; t < T; ++t) acc[i][t] = 0.f;
-            each_run([&](int unit, int a, int b) {
-                const bool shared = unit == n_units;
-                const int K = shared ? c.l.shared_inner : c.l.inner, ld = shared ? c.shared_row : c.row;
-                const float* w = reinterpret_cast<const float*>(shared ? c.l.shared_down : c.l.down) +
-                                 (shared ? 0 : (size_t)c.plan->expert[unit] * c.l.width * K);
-                const float* h = reinterpret_cast<const float*>(c.hidden) + (size_t)(shared ? c.max_units : unit) * c.T * c.row;
-                const float* rows[few::F32_ROWS];
+                for (int i = 0; i < 4; ++i) d[0][i] *= few::MX4_BACK;
+            if (mine && part == 0) {
+                // lane (g, t): features g (and g + 8 of a plain unit) of tokens 2 t and 2 t + 1
+                const int inner = shared ? c.l.shared_inner : c.l.inner, g = lane >> 2;
+                const bool gated = shared || c.l.gated;
 #pragma unroll
-                for (int i = 0; i < few::F32_ROWS; ++i) rows[i] = w + (size_t)min(n0 + r0 + i, c.l.width - 1) * K;
-                few::stream_f32<T>(rows, h, ld, shared ? (1u << c.T) - 1 : c.plan->tokens[unit], K, a, b, shared ? c.shared_wide : c.inner_wide,
-                                   true, acc);
-            });
-            put_four<T>(red[warp], r0, acc);
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 2 * (lane & 3) + (i & 1), feature = p.first + g + (i >> 1) * S::HALF;
+                    if ((gated && i > 1) || feature >= inner || !(users >> t & 1)) continue;
+                    put_hidden<KIND>(c, shared, p.unit, t, feature, unit_value(c, shared, d[0][i], d[0][i | 2], shared ? r.gate[t] : r.unit_weight[p.unit][t]));
+                }
+            }
         }
-    } else {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const int g = lane >> 2;
-        each_run([&](int unit, int a, int b) {
-            const bool shared = unit == n_units;
-            const int K = shared ? c.l.shared_inner : c.l.inner, ld = shared ? c.shared_row : c.row;
-            const bool live = g < c.T && (shared || (c.plan->tokens[unit] >> g & 1));
-            const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(c.hidden) + (size_t)(shared ? c.max_units : unit) * c.T * c.row * 2 +
-                                     (size_t)g * 2 * ld;
-            const size_t base = shared ? 0 : (size_t)c.plan->expert[unit] * c.l.width;
-            auto row = [&](int i) { return base + min(n0 + i, c.l.width - 1); };
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
-            tile_product<KIND == MX4, 2>(shared ? c.l.shared_down : c.l.down, shared ? c.l.shared_down_scales : c.l.down_scales, K, row,
-                                         live ? h : nullptr, live ? h + ld : nullptr, a, b, shared ? c.shared_wide : c.inner_wide, true, part);
-            // (only into the tokens that use the expert: zero times a weight that is not finite would reach the others)
-            const uint32_t users = shared ? 0xffu : c.plan->tokens[unit];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (users >> (2 * (lane & 3) + (i & 1)) & 1) acc[i] += part[i];
-        });
-        put_tile(red[warp], acc, KIND == MX4 ? few::MX4_BACK : 1.f);
+        // behind the last feature: zeros to the end of the row
+        const int inner = shared ? c.l.shared_inner : c.l.inner, row = shared ? c.shared_row : c.row;
+        if (mine && part == 0 && p.first + (shared ? S::HALF : features) >= inner)
+            for (int i = lane; i < (row - inner) * c.T; i += 32)
+                if (users >> (i % c.T) & 1) put_hidden<KIND>(c, shared, p.unit, i % c.T, inner + i / c.T, 0.f);
     }
-    __syncthreads();
-    const int f = threadIdx.x % 16, t = threadIdx.x / 16;
-    float sum = 0.f;
-    if (t < c.T)
-#pragma unroll
-        for (int s = 0; s < WARPS; ++s) sum += red[s].sum[f][t];
-    if (cluster > 1) {
-        if (rank > 0 && t < c.T) tc::st_cluster_f32(tc::map_to_rank(&others[rank - 1][f][t], 0), sum);
-        tc::cluster_arrive();
-        tc::cluster_wait();
-        if (rank > 0) return;
-        if (t < c.T)
-            for (int s = 1; s < cluster; ++s) sum += others[s - 1][f][t];
-    }
-    const int n = n0 + f;
-    if (t >= c.T || n >= c.l.width) return;
-    if (c.l.identity) {
-        const size_t at = (size_t)t * c.ldy + n;
-        const float y = KIND == F32 ? reinterpret_cast<const float*>(c.y)[at] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(c.y)[at]);
-        sum = fmaf(c.plan->own[t], y, sum);
-    }
-    c.out[(size_t)t * c.ldo + n] = sum + (c.residual ? c.residual[(size_t)t * c.ldr + n] : 0.f);
+    if (bars.gave_up && lane == 0) atomicOr(c.error_flag, 8);
 }
 
-template <typename K>
-int launch_clusters(K* kernel, int blocks, int cluster, size_t smem, cudaStream_t s, const Call& c, const char* what) {
+template <int KIND, int W>
+__global__ void __launch_bounds__(W * 32, 16 / W)
+down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
+    using S = Stream<KIND>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ Tile red[W], columns[W];
+    __shared__ Plan plan;
+    __shared__ Barriers<W> bars;
+    constexpr int STAGES = S::MOST_STAGES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    dd_launch_dependents();
+    if (c.l.shared_inner && c.inner_wide) ask_for(c.l.shared_down, matrix_bytes(KIND, c.l.width, c.l.shared_inner));
+    bars.init();
+    for (int i = lane; i < (int)(sizeof(Tile) / 4); i += 32) reinterpret_cast<float*>(&red[warp])[i] = 0.f;
+    dd_grid_wait();
+    // (all of it at once, used or not)
+    for (int i = threadIdx.x; i < (int)(sizeof(Plan) / 4); i += W * 32) reinterpret_cast<uint32_t*>(&plan)[i] = reinterpret_cast<const uint32_t*>(c.plan)[i];
+    __syncthreads();
+    const int n0 = blockIdx.x * S::ROWS;
+    // the result's row and column of this thread, and what the sum is added to
+    const int f = threadIdx.x % S::ROWS, t = threadIdx.x / S::ROWS, column = n0 + f;
+    const bool live = t < c.T && column < c.l.width;
+    float result = live && c.residual ? c.residual[(size_t)t * c.ldr + column] : 0.f;
+    if (live && c.l.identity) {
+        const size_t at = (size_t)t * c.ldy + column;
+        const float y = KIND == F32 ? reinterpret_cast<const float*>(c.y)[at] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(c.y)[at]);
+        result = fmaf(plan.own[t], y, result);
+    }
+    auto steps_of = [](int K) { return (K + S::STEP - 1) / S::STEP; };
+    const int for_shared = steps_of(c.l.shared_inner), per_unit = steps_of(c.l.inner);
+    const int total = for_shared + plan.n_units * per_unit;
+    const int from = (int)((long long)total * warp / W), to = (int)((long long)total * (warp + 1) / W);
+    // step -> unit (-1: the shared one), its first step and its end
+    auto unit_of = [&](int at) { return at < for_shared ? -1 : (at - for_shared) / per_unit; };
+    auto begin_of = [&](int unit) { return unit < 0 ? 0 : for_shared + unit * per_unit; };
+    auto row_of = [&](int unit) { return (unit < 0 ? 0 : plan.expert[unit] * c.l.width) + n0; };
+    Ring<KIND> ring(bars.full[warp], tc::smem_u32(smem) + warp * STAGES * S::STAGE_BYTES, STAGES);
+    int f_at = from, f_begin = 0, f_end = from, f_row = 0;
+    bool f_shared = false;
+    auto fetch = [&] {
+        if (f_at >= to) return;
+        if (f_at == f_end) {
+            const int unit = unit_of(f_at);
+            f_shared = unit < 0;
+            f_begin = begin_of(unit);
+            f_end = begin_of(unit + 1);
+            f_row = row_of(unit);
+        }
+        if (c.inner_wide && lane == 0)
+            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, f_row, f_row + S::HALF);
+        ring.next_asked();
+        ++f_at;
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) fetch();
+    for (int at = from; at < to;) {               // the runs of steps of one unit
+        const int unit = unit_of(at), begin = begin_of(unit), end = min(to, begin_of(unit + 1));
+        const bool shared = unit < 0;
+        const int K = shared ? c.l.shared_inner : c.l.inner, ld = shared ? c.shared_row : c.row;
+        const uint32_t users = shared ? (1u << c.T) - 1 : plan.tokens[unit], list = list_of(users);
+        const int n = __popc(users);
+        const size_t hidden = (size_t)(shared ? c.max_units : unit) * c.T * c.row, matrix_rows = (size_t)(shared ? 1 : c.l.experts) * c.l.width;
+        const void* matrix = shared ? c.l.shared_down : c.l.down;
+        const int first_row = row_of(unit);
+        auto next = [&](int s) {
+            const uint32_t place = ring.take(c.inner_wide, &bars.gave_up);
+            if (!c.inner_wide) fill_stage<KIND>(place, matrix, first_row, first_row + S::HALF, matrix_rows, K, s - begin);
+            return place;
+        };
+        if constexpr (KIND == F32)
+            by_count(n, [&](auto count) {
+                constexpr int N = decltype(count)::value;
+                unsigned long long d[few::F32_ROWS][N] = {};
+                for (int s = at; s < end; ++s) {
+                    fma_step<N>(next(s), reinterpret_cast<const float*>(c.hidden) + hidden, ld, list, s - begin, d);
+                    __syncwarp();
+                    fetch();
+                }
+                put_rows<N, true>(red[warp], 0, list, n, d);
+            });
+        else {
+            const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(c.hidden) + hidden * TERMS;
+            // columns: the terms of the first token of the list, of the second, ...
+            auto columns_by = [&](auto count) {
+                constexpr int P = decltype(count)::value, Q = PIECES<KIND>;
+                // (columns beyond the last term read the first one; nobody looks at them)
+                const __nv_bfloat16* x[P];
+                float d[P][4] = {};
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const int q = p * few::COLUMNS + g < n * TERMS ? p * few::COLUMNS + g : 0;
+                    x[p] = h + (size_t)(listed(list, q / TERMS) * TERMS + q % TERMS) * ld;
+                }
+                const uint32_t *s0 = nullptr, *s1 = nullptr;
+                uint32_t four0 = 0, four1 = 0;
+                if (KIND == MX4) {
+                    const size_t groups = steps_of(K), last = matrix_rows - 1;
+                    const uint32_t* scales = reinterpret_cast<const uint32_t*>(shared ? c.l.shared_down_scales : c.l.down_scales);
+                    s0 = scales + min((size_t)first_row + g, last) * groups;
+                    s1 = scales + min((size_t)first_row + g + 8, last) * groups;
+                    four0 = s0[at - begin]; four1 = s1[at - begin];
+                }
+                // a step's columns and scales are requested a step ahead where there are registers for it
+                constexpr int AHEAD = P * Q <= 4 ? 1 : 0;
+                uint4 b[AHEAD + 1][P][Q];
+                if (AHEAD)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) take_column<KIND>(b[0][p], x[p], at - begin);
+                for (int s = at; s < end; s += AHEAD + 1)
+#pragma unroll
+                    for (int u = 0; u <= AHEAD; ++u) {
+                        if (s + u >= end) break;
+                        const int soon = s + u + AHEAD - begin, v = (u + AHEAD) & AHEAD;
+                        if (s + u + AHEAD < end) {
+#pragma unroll
+                            for (int p = 0; p < P; ++p) take_column<KIND>(b[v][p], x[p], soon);
+                        }
+                        uint32_t n0 = 0, n1 = 0;
+                        if (KIND == MX4 && s + u + 1 < end) { n0 = s0[s + u + 1 - begin]; n1 = s1[s + u + 1 - begin]; }
+                        mma_step<KIND, P>(next(s + u), four0, four1, b[u], d);
+                        four0 = n0; four1 = n1;
+                        __syncwarp();
+                        fetch();
+                    }
+                // into the tokens that use the expert (the others are not touched: zero times a weight that is not finite is no zero)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    put_tile<KIND>(columns[warp], d[p]);
+                    __syncwarp();
+                    if (lane < 16)
+                        for (int i = 0; i < few::COLUMNS && p * few::COLUMNS + i < n * TERMS; ++i)
+                            red[warp].sum[lane][listed(list, (p * few::COLUMNS + i) / TERMS)] += columns[warp].sum[lane][i];
+                    __syncwarp();
+                }
+            };
+            if (n * TERMS <= few::COLUMNS) columns_by(Count<1>{});
+            else if (n * TERMS <= 2 * few::COLUMNS) columns_by(Count<2>{});
+            else columns_by(Count<3>{});
+        }
+        at = end;
+    }
+    __syncthreads();
+    if (bars.gave_up && threadIdx.x == 0) atomicOr(c.error_flag, 8);
+    if (!live) return;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < W; ++s) sum += red[s].sum[f][t];
+    c.out[(size_t)t * c.ldo + column] = sum + result;
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A matrix of the layer as TMA boxes of its kind (Stream); one whose rows are no whole 16-byte pieces has none.
+template <int KIND>
+int layer_map(CUtensorMap* map, const void* base, long long rows, int K) {
+    using S = Stream<KIND>;
+    const long long row_bytes = KIND == MX4 ? (long long)dd_ceil_div(K, mx4::GROUP) * mx4::GROUP_BYTES : (long long)K * S::ELEMENT;
+    if (!base || rows <= 0 || row_bytes % 16 || ((uintptr_t)base & 15)) return 0;
+    static EncodeTiled enc = nullptr;
+    if (!enc) {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            enc = reinterpret_cast<EncodeTiled>(sym);
+    }
+    if (!enc) return dd_fail("dd_moe_tokens: cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {(cuuint64_t)(KIND == MX4 ? row_bytes : K), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {(cuuint32_t)S::BOX_WIDTH, (cuuint32_t)S::HALF};
+    cuuint32_t elem[2] = {1, 1};
+    const CUresult r = enc(map, KIND == F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KIND == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                           2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : KIND == BF16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return dd_fail("dd_moe_tokens: cannot describe a matrix of %lld x %d to TMA (driver error %d)", rows, K, (int)r);
+    return 0;
+}
+template <int KIND>
+int layer_maps(Maps* m, const DdExpertLayer& l) {
+    if (int e = layer_map<KIND>(&m->gate_up, l.gate_up, (long long)l.experts * l.inner * (l.gated ? 2 : 1), l.width)) return e;
+    if (int e = layer_map<KIND>(&m->down, l.down, (long long)l.experts * l.width, l.inner)) return e;
+    if (int e = layer_map<KIND>(&m->shared_gate_up, l.shared_gate_up, 2ll * l.shared_inner, l.width)) return e;
+    return layer_map<KIND>(&m->shared_down, l.shared_down, l.width, l.shared_inner);
+}
+
+template <int KIND>
+int launch_up(const Call& c, const Maps& m, int blocks, size_t smem, cudaStream_t s) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(blocks);
-    config.blockDim = dim3(THREADS);
+    config.blockDim = dim3(UP_THREADS);
     config.dynamicSmemBytes = smem;
     config.stream = s;
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim.x = cluster;
+    attrs[0].val.clusterDim.x = c.cluster;
     attrs[0].val.clusterDim.y = 1;
     attrs[0].val.clusterDim.z = 1;
     attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attrs;
     config.numAttrs = dd_pdl_enabled ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, c);
-    if (e != cudaSuccess) return dd_fail("dd_moe_tokens (%s, clusters of %d): %s", what, cluster, cudaGetErrorString(e));
+    cudaError_t e = cudaFuncSetAttribute(up_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, up_kernel<KIND>, c, m);
+    if (e != cudaSuccess) return dd_fail("dd_moe_tokens (clusters of %d, %d bytes of shared memory): %s", c.cluster, (int)smem, cudaGetErrorString(e));
+    return dd_check_launch("dd_moe_tokens");
+}
+template <int KIND, int W>
+int launch_down(const Call& c, const Maps& m, int tiles, cudaStream_t s) {
+    constexpr int BYTES = W * Stream<KIND>::MOST_STAGES * Stream<KIND>::STAGE_BYTES + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(down_kernel<KIND, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e != cudaSuccess) return dd_fail("dd_moe_tokens: shared memory of %d bytes refused: %s", BYTES, cudaGetErrorString(e));
+    dd_launch(down_kernel<KIND, W>, dim3(tiles), dim3(W * 32), (size_t)BYTES, s, c, m);
     return dd_check_launch("dd_moe_tokens");
 }
 
-template <int KIND, int T>
-int launch_both(Call& c, int sms, cudaStream_t s) {
+template <int KIND>
+int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
+    using S = Stream<KIND>;
     const int outputs = c.l.experts + c.l.identity, rows = outputs + c.l.shared_gate;
     // a router of up to 64 KB is read by every block for itself, a larger one shared by a cluster's blocks
-    const size_t router_bytes = c.l.router ? (size_t)rows * c.l.width * (KIND == F32 ? 4 : 2) : 0;
-    c.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) ? 4 : 8;
-    const int tiles = (rows + 15) / 16, shares = tiles < WARPS ? WARPS / tiles : 1;
-    const size_t smem = !c.l.router ? 0 : sizeof(Tile) * tiles * shares + sizeof(float) * (c.cluster * tiles * 16 * MAX_TOKENS +
-                                                                                             MAX_TOKENS * (2 * outputs + c.l.groups));
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(up_kernel<KIND, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return dd_fail("dd_moe_tokens: shared memory of %d bytes refused: %s", (int)smem, cudaGetErrorString(e));
-    }
-    const int tile_rows = c.l.gated ? 8 : 16;
-    const long long tasks = (long long)c.max_units * ((c.l.inner + tile_rows - 1) / tile_rows) + (c.l.shared_inner + 7) / 8;
-    const int most = sms * 2 / c.cluster * c.cluster;
-    int blocks = tasks < most ? (int)((tasks + c.cluster - 1) / c.cluster * c.cluster) : most;
-    if (int e = launch_clusters(up_kernel<KIND, T>, blocks, c.cluster, smem, s, c, "up")) return e;
-    const int rows16 = dd_ceil_div(c.l.width, 16);
-    c.cluster = rows16 >= 2 * sms ? 1 : rows16 >= sms ? 2 : 4;
-    return launch_clusters(down_kernel<KIND, T>, rows16 * c.cluster, c.cluster, 0, s, c, "down");
+    // (128 outputs and more leave no room for what eight blocks send)
+    const size_t router_bytes = c.l.router ? (size_t)rows * c.l.width * S::ELEMENT : 0;
+    const int tiles = (rows + 15) / 16, shares = tiles < UP_WARPS ? UP_WARPS / tiles : 1;
+    c.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) || tiles > 8 ? 4 : 8;
+    const size_t scratch = !c.l.router ? 0 : sizeof(Tile) * tiles * shares + sizeof(float) * (c.cluster * tiles * 16 * MAX_TOKENS +
+                                                                                                MAX_TOKENS * (2 * outputs + (c.l.groups > MAX_TOP ? c.l.groups : MAX_TOP)));
+    c.y_pitch = dd_ceil_div((long long)c.l.width, 128) * 128 * S::ELEMENT + 16;
+    constexpr size_t MOST = 227 * 1024 - 32 * 1024;      // less the static part
+    const size_t fixed = scratch + (size_t)c.T * c.y_pitch + 1024, stage = UP_WARPS * S::STAGE_BYTES;
+    if (fixed + 2 * stage > MOST)
+        return dd_fail("dd_moe_tokens: %d rows of %d elements are more than a block's shared memory holds beside its rings", c.T, c.l.width);
+    c.stages = (int)((MOST - fixed) / stage);
+    if (c.stages > S::MOST_STAGES) c.stages = S::MOST_STAGES;
+    // what the GPU holds at once, a block an SM (a second wave of blocks would double the time): a B200's SMs take 33 clusters
+    // of four, 15 of eight
+    const int most = sms >= 148 ? (c.cluster == 1 ? sms : c.cluster == 4 ? 132 : 120) : sms / 2 / c.cluster * c.cluster;
+    const int features = c.l.gated ? S::HALF : S::ROWS;
+    const long long at_most = (long long)c.max_units * ((c.l.inner + features - 1) / features) + (c.l.shared_inner + S::HALF - 1) / S::HALF;
+    if (at_most * UP_WARPS > INT_MAX || (long long)c.l.experts * c.l.inner * 2 > INT_MAX || (long long)c.l.experts * c.l.width > INT_MAX)
+        return dd_fail("dd_moe_tokens: %d experts of %d x %d are too large", c.l.experts, c.l.inner, c.l.width);
+    const int blocks = at_most < most ? (int)((at_most + c.cluster - 1) / c.cluster * c.cluster) : most;
+    if (int e = launch_up<KIND>(c, m, blocks, fixed + c.stages * stage, s)) return e;
+    // a block a tile; as many warps on it as let all blocks run at once
+    const int down_tiles = dd_ceil_div(c.l.width, S::ROWS);
+    if (down_tiles <= sms) return launch_down<KIND, 16>(c, m, down_tiles, s);
+    if (down_tiles <= 2 * sms) return launch_down<KIND, 8>(c, m, down_tiles, s);
+    return launch_down<KIND, 4>(c, m, down_tiles, s);
 }
 
-int hidden_row(int inner) { return (inner + 7) / 8 * 8; }
+int hidden_row(int kind, int inner) { return (inner + step_of(kind) - 1) / step_of(kind) * step_of(kind); }
 size_t hidden_bytes(const DdExpertLayer& l, int T, int max_units) {
-    return (size_t)T * 4 * ((size_t)max_units * hidden_row(l.inner) + hidden_row(l.shared_inner));
+    return (size_t)T * (l.kind == F32 ? 4 : 2 * TERMS) * ((size_t)max_units * hidden_row(l.kind, l.inner) + hidden_row(l.kind, l.shared_inner));
 }
 int units_of(const DdExpertLayer& l, int T) { return T * l.top < l.experts ? T * l.top : l.experts; }
 }  // namespace
@@ -474,38 +907,48 @@ int units_of(const DdExpertLayer& l, int T) { return T * l.top < l.experts ? T *
 DD_API long long dd_moe_tokens_scratch(const DdExpertLayer* l, int T) {
     return (long long)(sizeof(Plan) + hidden_bytes(*l, T, units_of(*l, T)));
 }
+// The layer's matrices as TMA takes them: 512 bytes, 64-byte aligned, which every call copies. They hold while the matrices lie where they are.
+DD_API int dd_moe_tokens_maps(const DdExpertLayer* l, void* maps) {
+    static_assert(sizeof(Maps) == 512, "four tensor maps");
+    Maps* m = (Maps*)maps;
+    return l->kind == F32 ? layer_maps<F32>(m, *l) : l->kind == BF16 ? layer_maps<BF16>(m, *l) : layer_maps<MX4>(m, *l);
+}
 
 // y [T, ldy] (float32 or bfloat16, by the layer's kind), residual [T, ldr] float32 or null, out [T, ldo] float32 (may be
 // residual), ids [T] with a table. An expert or a token id out of range sets error bit 1 and is left out.
-DD_API int dd_moe_tokens(const DdExpertLayer* l, const void* y, int ldy, const float* residual, int ldr, float* out, int ldo, const int* ids,
-                         int T, void* scratch, int sms, int* error_flag, void* stream) {
+DD_API int dd_moe_tokens(const DdExpertLayer* l, const void* maps, const void* y, int ldy, const float* residual, int ldr, float* out, int ldo,
+                         const int* ids, int T, void* scratch, int sms, int* error_flag, void* stream) {
     if (T <= 0) return 0;
     const int outputs = l->experts + l->identity;
     if (T > MAX_TOKENS || l->top <= 0 || l->top > MAX_TOP || l->experts <= 0 || outputs + l->shared_gate > MAX_OUTPUTS || l->top > outputs)
         return dd_fail("dd_moe_tokens: %d tokens (at most %d), %d of %d experts (at most %d of %d)", T, MAX_TOKENS, l->top, outputs, MAX_TOP,
                        MAX_OUTPUTS);
+    if (l->kind == MX4) {
+        const void* codes[4] = {l->gate_up, l->down, l->shared_gate_up, l->shared_down};
+        const void* scales[4] = {l->gate_up_scales, l->down_scales, l->shared_gate_up_scales, l->shared_down_scales};
+        for (int i = 0; i < 4; ++i)
+            if (((uintptr_t)codes[i] & 15) || ((uintptr_t)scales[i] & 3)) return dd_fail("dd_moe_tokens: 4-bit matrices must be 16-byte aligned");
+    }
     if (!l->router == !l->table || (l->table && !ids)) return dd_fail("dd_moe_tokens: a router, or a table with token ids");
     if (l->groups <= 0 || outputs % l->groups || l->keep <= 0 || l->keep > l->groups || l->width <= 0 || l->inner <= 0)
         return dd_fail("dd_moe_tokens: %d experts in %d groups of which %d stay, width %d, inner %d", outputs, l->groups, l->keep, l->width, l->inner);
     Call c;
     c.l = *l; c.y = y; c.residual = residual; c.out = out; c.ids = ids; c.error_flag = error_flag; c.T = T; c.ldy = ldy; c.ldr = ldr; c.ldo = ldo;
     c.max_units = units_of(*l, T);
-    c.row = hidden_row(l->inner); c.shared_row = hidden_row(l->shared_inner);
+    c.row = hidden_row(l->kind, l->inner); c.shared_row = hidden_row(l->kind, l->shared_inner);
     c.plan = (Plan*)scratch;
     c.hidden = (uint8_t*)scratch + sizeof(Plan);
     const int piece = l->kind == F32 ? 4 : 8;
     auto aligned = [](const void* p) { return !((uintptr_t)p & 15); };
-    c.w_wide = l->width % piece == 0 && aligned(l->gate_up) && aligned(l->shared_gate_up) && aligned(l->router) &&
-               (!l->router || l->router_stride % piece == 0);
-    c.inner_wide = l->inner % piece == 0 && aligned(l->down);
-    c.shared_wide = l->shared_inner % piece == 0 && aligned(l->shared_down);
+    const bool four = l->kind == MX4;            // (whose rows always are whole pieces)
+    c.router_wide = l->width % piece == 0 && aligned(l->router) && l->router_stride % piece == 0;
+    c.w_wide = four || (l->width % piece == 0 && aligned(l->gate_up) && aligned(l->shared_gate_up));
+    c.inner_wide = four || (l->inner % piece == 0 && l->shared_inner % piece == 0 && aligned(l->down) && aligned(l->shared_down));
     c.y_wide = l->width % piece == 0 && ldy % piece == 0 && aligned(y);
     cudaStream_t s = (cudaStream_t)stream;
-    if (l->kind == BF16) return launch_both<BF16, 8>(c, sms, s);
-    if (l->kind == MX4) return launch_both<MX4, 8>(c, sms, s);
-    if (l->kind != F32) return dd_fail("dd_moe_tokens: unknown kind %d", l->kind);
-    if (T == 1) return launch_both<F32, 1>(c, sms, s);
-    if (T == 2) return launch_both<F32, 2>(c, sms, s);
-    if (T <= 4) return launch_both<F32, 4>(c, sms, s);
-    return launch_both<F32, 8>(c, sms, s);
+    const Maps& m = *(const Maps*)maps;
+    if (l->kind == BF16) return launch_both<BF16>(c, m, sms, s);
+    if (l->kind == MX4) return launch_both<MX4>(c, m, sms, s);
+    if (l->kind == F32) return launch_both<F32>(c, m, sms, s);
+    return dd_fail("dd_moe_tokens: unknown kind %d", l->kind);
 }

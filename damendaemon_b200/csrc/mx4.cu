@@ -135,8 +135,8 @@ gemm_mx4_rows_kernel(const RowsParams p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = min(from + u, p.groups - 1);       // groups past the share are not used
-            c0[u] = __ldg(w0 + at * 4); c1[u] = __ldg(w1 + at * 4);
-            f0[u] = __ldg(s0 + at); f1[u] = __ldg(s1 + at);
+            c0[u] = w0[at * 4]; c1[u] = w1[at * 4];
+            f0[u] = s0[at]; f1[u] = s1[at];
         }
     };
     dd_launch_dependents();
@@ -259,6 +259,7 @@ DD_API int dd_gemm_mx4_rows(const void* X, int ldx, const void* codes, const voi
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return dd_fail("dd_gemm_mx4_rows: K=%d", K);
     if (out_dtype != DD_BF16 && out_dtype != DD_F32) return dd_fail("dd_gemm_mx4_rows: unknown output dtype %d", out_dtype);
+    if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 3)) return dd_fail("dd_gemm_mx4_rows: the 4-bit matrix must be 16-byte aligned");
     if (M > 65535 * 16) return dd_fail("dd_gemm_mx4_rows: %d rows", M);
     RowsParams p;
     p.codes = (const uint32_t*)codes; p.scales = (const uint32_t*)scales; p.X = (const __nv_bfloat16*)X; p.bias = bias;

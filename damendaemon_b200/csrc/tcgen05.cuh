@@ -207,6 +207,12 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, uint32_t a, uint
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// One value into the block that `addr` and `bar` (addresses from map_to_rank) belong to; its four bytes are counted on the
+// barrier there. No fence and no barrier of the cluster: what else this block has in flight is not waited for.
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(addr), "f"(v), "r"(bar) : "memory");
+}
+
 // ---- two SMs on one tile (cta_group::2): the blocks of a cluster of two; rank 0 issues the MMAs ----
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(columns) : "memory");

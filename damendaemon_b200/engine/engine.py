@@ -52,11 +52,17 @@ def require_cuda(device):
 class Engine:
     def __init__(self, model_dir=None, *, config=None, tensors=None, dtype="bfloat16", kv_tokens=None,
                  page_size=16, max_requests=64, device="cuda:0", gemm="auto", check_device_errors=True,
-                 use_graph=False, max_context=None):
+                 use_graph=False, max_context=None, feed_forward="auto"):
         """Either ``model_dir`` (config.json + model.safetensors) or ``config`` (the raw
         config.json dict) with ``tensors`` ({checkpoint name: tensor}). ``max_context``: most tokens a
         request may hold, at most the model's positions; for an architecture that names no limit the
-        default is the cache's size in tokens, or ``UNBOUNDED_CONTEXT`` without one."""
+        default is the cache's size in tokens, or ``UNBOUNDED_CONTEXT`` without one. ``feed_forward``: 'auto', or 'mx4' to hold the
+        matrices of the feed-forwards in microscaled 4-bit numbers (17/32 of a byte an element; a bfloat16 engine's; what they
+        were is rounded when the engine is built, their products are as exact as others)."""
+        if feed_forward not in ("auto", "mx4"):
+            raise ValueError(f"feed_forward {feed_forward!r} is not supported; known: ['auto', 'mx4']")
+        if feed_forward == "mx4" and (DTYPES[dtype] != torch.bfloat16 or gemm == "simt"):
+            raise ValueError("4-bit feed-forwards belong to a bfloat16 engine with tensor cores (dtype 'bfloat16', gemm not 'simt')")
         self.device = require_cuda(device)
         torch.cuda.set_device(self.device)
         self.dtype = DTYPES[dtype]
@@ -74,12 +80,12 @@ class Engine:
             weights = load_weights(model_dir, self.spec, decls, self.dtype, self.device)
         else:
             weights = check_and_place(DictSource(tensors), self.spec, decls, self.dtype, self.device)
-        self.runtime = Runtime(dtype=self.dtype, device=self.device, gemm=gemm, page_size=page_size)
+        self.runtime = Runtime(dtype=self.dtype, device=self.device, gemm=gemm, page_size=page_size, feed_forward=feed_forward)
         kernels.library("core")
         if self.dtype == torch.bfloat16 and gemm != "simt":
             kernels.library("tensor")
         self.model = DecoderModel(self.spec, weights, self.runtime)
-        self.weight_bytes = sum(t.numel() * t.element_size() for t in weights.values())
+        self.weight_bytes = sum(t.nbytes for t in weights.values())
         self.page_size = page_size
         limit = self.spec.max_positions
         if limit is None:

@@ -104,7 +104,8 @@ _SIGNATURES = {
         "dd_post_norm": [_c_void, _c_void, _c_void, _c_float, _c_float, _c_void, _c_int, _c_void, _c_float, _c_float, _c_void, _c_int,
                          _c_int, _c_int, _c_void],
         "dd_round_rows": [_c_void, _c_void, ctypes.c_longlong, _c_void],
-        "dd_moe_tokens": [_c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
+        "dd_moe_tokens_maps": [_c_void, _c_void],
+        "dd_moe_tokens": [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
         "dd_mx4_quantize": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_int, _c_void],
         "dd_mx4_values": [_c_void, _c_void, ctypes.c_longlong, _c_int, _c_void, _c_int, _c_void],
         "dd_gemm_mx4_rows": [_c_void, _c_int] + [_c_void] * 4 + [_c_int, _c_void] + [_c_int] * 6 + [_c_void],
@@ -1602,7 +1603,15 @@ class ExpertLayer:
                 any(m.device.index != self.device_index for m in matrices):
             raise KernelError("expert layer: its tensors are on more than one device")
         self._at = ctypes.addressof(raw)
+        self._map_store = ctypes.create_string_buffer(512 + 64)      # the matrices as TMA takes them, at a 64-byte boundary
+        self._maps = (ctypes.addressof(self._map_store) + 63) // 64 * 64
+        _call(library("core"), "dd_moe_tokens_maps", self._at, self._maps, n_kernels=0)
         self._scratch = [0] + [int(library("core").dd_moe_tokens_scratch(self._at, t)) for t in range(1, MOE_TOKENS + 1)]
+
+
+def expert_layer_fits(top, router_rows):
+    """Whether moe_tokens chooses among that many router rows (experts, identity outputs, a shared unit's gate)."""
+    return top <= MOE_TOP and router_rows <= MOE_OUTPUTS
 
 
 def moe_tokens(layer, y, residual=None, ids=None, out=None):
@@ -1626,7 +1635,7 @@ def moe_tokens(layer, y, residual=None, ids=None, out=None):
     if T == 0:
         return out
     scratch = torch.empty(layer._scratch[T], dtype=torch.uint8, device=y.device)
-    _call(library("core"), "dd_moe_tokens", layer._at, pointer, y.stride(0), _ptr(residual, "residual", torch.float32),
+    _call(library("core"), "dd_moe_tokens", layer._at, layer._maps, pointer, y.stride(0), _ptr(residual, "residual", torch.float32),
           0 if residual is None else residual.stride(0), _ptr(out, "out", torch.float32), out.stride(0), _ptr(ids, "ids"), T, scratch.data_ptr(),
           sm_count(y.device), _ptr(error_flag(y.device)), _stream(), n_kernels=2)
     return out

@@ -3,18 +3,52 @@ epilogue and the residual add into the second's (damendaemon/gpt2.py:62-64). Exp
 table of token ids: small gated units, a token's chosen ones weighted equally, a shared one for every
 token; their products run grouped, expert by expert, over rows sorted on the device. Experts chosen
 by a router's scores: the same grouped products after a routing kernel, each chosen expert's output, or its input, weighted
-by its score; the experts are gated units or plain ones of two matrices. 'gated': one dense gated unit. 'none': a layer without a feed-forward."""
+by its score; the experts are gated units or plain ones of two matrices. 'gated': one dense gated unit. 'none': a layer without a feed-forward.
+A step of a few tokens runs a whole expert layer in two kernels. With the runtime's ``feed_forward`` 'mx4' every matrix of a
+feed-forward becomes microscaled 4-bit numbers when the part is built (the router stays as it is)."""
 from __future__ import annotations
 
 import torch
 
 from .. import kernels
 from .interfaces import FeedForward
-from .linear import grouped_gated_unit, grouped_linear, grouped_on_tensor_cores, grouped_tile, linear
+from .linear import grouped_gated_unit, grouped_linear, grouped_on_tensor_cores, grouped_tile, linear, splits_float32
 from .registry import register_feed_forward
 from .spec import PlainUnitSpec, TensorDecl
 
 ACTIVATIONS = ("gelu_new", "gelu", "relu2")
+
+
+def _held(runtime, w):
+    """A feed-forward's matrix, or stack of matrices, as the runtime wants it held."""
+    if runtime.feed_forward != "mx4" or isinstance(w, kernels.Mx4Matrix):
+        return w
+    return kernels.mx4_quantize(w)
+
+
+def _take(runtime, weights, name):
+    """The matrix of that name; its held form takes its place among the weights."""
+    weights[name] = _held(runtime, weights[name])
+    return weights[name]
+
+
+def _stacked(runtime, weights, experts, names):
+    """The experts' matrices of these names, one expert's under one another, as one stack (they leave the weights: one copy on the
+    device, and in the engine's count of bytes)."""
+    stack = torch.stack([torch.cat([weights[n] for n in names(u)], dim=0) for u in experts])
+    for u in experts:
+        for n in names(u):
+            weights.pop(n, None)
+    return _held(runtime, stack)
+
+
+def _few_tokens(runtime, gate_up, down, **options):
+    """The layer as kernels.moe_tokens takes it, or None where the kernels of larger steps serve these too: a runtime that
+    wants the kernels whose rows do not depend on what is beside them, float32 matrices of a size whose products keep a row's
+    bits for the same reason (splits_float32), or more experts than a block chooses among."""
+    if runtime.gemm == "simt" or (runtime.dtype == torch.float32 and not splits_float32(*down.shape[1:])) or not kernels.expert_layer_fits(options.get("top"), gate_up.shape[0] + options.get("identity", 0) + 1):
+        return None
+    return kernels.ExpertLayer(gate_up, down, **options)
 
 
 @register_feed_forward("dense")
@@ -25,7 +59,7 @@ class DenseFeedForward(FeedForward):
         if spec.activation not in ACTIVATIONS:
             raise ValueError(f"activation {spec.activation!r} is not supported; known: {ACTIVATIONS}")
         self.spec, self.runtime = spec, runtime
-        self.up_w, self.down_w = weights[spec.up_weight], weights[spec.down_weight]
+        self.up_w, self.down_w = _take(runtime, weights, spec.up_weight), _take(runtime, weights, spec.down_weight)
         self.up_b = weights[spec.up_bias] if spec.up_bias else None
         self.down_b = weights[spec.down_bias] if spec.down_bias else None
 
@@ -87,19 +121,12 @@ class TableRoutedExperts(FeedForward):
             raise ValueError(f"{spec.top} experts per token of {len(spec.experts)}")
         self.table = weights[spec.table]
         self.tensor_cores = grouped_on_tensor_cores(runtime, runtime.dtype, spec.width, first.inner)
-        self.gate_up = torch.stack([torch.cat([weights[u.gate_weight], weights[u.up_weight]], dim=0) for u in spec.experts])
-        self.down = torch.stack([weights[u.down_weight] for u in spec.experts])
-        # the stacks take the place of the single matrices (one copy on the device, and in the engine's count of bytes)
-        for u in spec.experts:
-            for name in (u.gate_weight, u.up_weight, u.down_weight):
-                weights.pop(name, None)
+        self.gate_up = _stacked(runtime, weights, spec.experts, lambda u: (u.gate_weight, u.up_weight))
+        self.down = _stacked(runtime, weights, spec.experts, lambda u: (u.down_weight,))
         weights[spec.table + ":gate_up"], weights[spec.table + ":down"] = self.gate_up, self.down
-        self.shared = None
-        if spec.shared is not None:
-            u = spec.shared
-            joined = torch.cat([weights.pop(u.gate_weight), weights.pop(u.up_weight)], dim=0).contiguous()
-            weights[spec.table + ":shared_gate_up"] = joined
-            self.shared = (joined, weights[u.down_weight])
+        self.shared = _shared_unit(runtime, weights, spec.shared, spec.table)
+        self.few = _few_tokens(runtime, self.gate_up, self.down, top=spec.top, table=self.table, gated=_gated(first),
+                               shared=self.shared, shared_gated=_gated(spec.shared))
 
     @staticmethod
     def tensor_decls(spec):
@@ -113,6 +140,8 @@ class TableRoutedExperts(FeedForward):
     def forward(self, y, residual, ctx):
         s, rt = self.spec, self.runtime
         unit = s.experts[0]
+        if self.few is not None and y.shape[0] <= kernels.MOE_TOKENS:
+            return kernels.moe_tokens(self.few, y, residual, ids=ctx.token_ids, out=residual)
         if self.shared is not None:
             gate_up = linear(rt, y, self.shared[0])
             hidden = kernels.gated_unit(gate_up, s.shared.limit, s.shared.alpha, form=s.shared.activation)
@@ -125,6 +154,19 @@ class TableRoutedExperts(FeedForward):
         hidden = grouped_gated_unit(self.tensor_cores, rows, self.gate_up, tile_group, tile, unit.limit, unit.alpha, unit.activation)
         out = grouped_linear(self.tensor_cores, hidden, self.down, tile_group, tile, out_dtype=torch.float32)
         return kernels.combine_rows(out, pair_row, residual, s.top, 1.0 / s.top)
+
+
+def _gated(unit):
+    """A gated unit's numbers as the kernels take them; None for a plain unit, or none at all."""
+    return None if unit is None or isinstance(unit, PlainUnitSpec) else (unit.limit or 0.0, unit.alpha, unit.activation)
+
+
+def _shared_unit(runtime, weights, unit, key):
+    if unit is None:
+        return None
+    joined = _held(runtime, torch.cat([weights.pop(unit.gate_weight), weights.pop(unit.up_weight)], dim=0).contiguous())
+    weights[key + ":shared_gate_up"] = joined
+    return joined, _take(runtime, weights, unit.down_weight)
 
 
 def _unit_form(unit):
@@ -152,8 +194,8 @@ class GatedFeedForward(FeedForward):
     def __init__(self, spec, weights, runtime):
         self.spec, self.runtime = spec, runtime
         _check_unit(spec.unit)
-        self.gate_up = weights[spec.unit.gate_weight + "+" + spec.unit.up_weight]
-        self.down = weights[spec.unit.down_weight]
+        self.gate_up = _take(runtime, weights, spec.unit.gate_weight + "+" + spec.unit.up_weight)
+        self.down = _take(runtime, weights, spec.unit.down_weight)
 
     @staticmethod
     def tensor_decls(spec):
@@ -210,19 +252,15 @@ class ScoreRoutedExperts(FeedForward):
         self.tensor_cores = grouped_on_tensor_cores(runtime, runtime.dtype, spec.width, first.inner)
         # plain units: the up matrices alone
         gates = (lambda u: ()) if self.plain else (lambda u: (u.gate_weight,))
-        self.gate_up = torch.stack([torch.cat([weights[n] for n in (*gates(u), u.up_weight)], dim=0) for u in spec.experts])
-        self.down = torch.stack([weights[u.down_weight] for u in spec.experts])
-        # the stacks take the place of the single matrices (one copy on the device, and in the engine's count of bytes)
-        for u in spec.experts:
-            for name in (*gates(u), u.up_weight, u.down_weight):
-                weights.pop(name, None)
+        self.gate_up = _stacked(runtime, weights, spec.experts, lambda u: (*gates(u), u.up_weight))
+        self.down = _stacked(runtime, weights, spec.experts, lambda u: (u.down_weight,))
         weights[spec.router + ":gate_up"], weights[spec.router + ":down"] = self.gate_up, self.down
-        self.shared = None
-        if spec.shared is not None:
-            u = spec.shared
-            joined = torch.cat([weights.pop(u.gate_weight), weights.pop(u.up_weight)], dim=0).contiguous()
-            weights[spec.router + ":shared_gate_up"] = joined
-            self.shared = (joined, weights[u.down_weight])
+        self.shared = _shared_unit(runtime, weights, spec.shared, spec.router)
+        self.few = _few_tokens(runtime, self.gate_up, self.down, top=spec.top, router=self.router, gated=_gated(first),
+                               activation=first.activation if self.plain else None, softmax=spec.score == "softmax", groups=spec.groups,
+                               keep=spec.keep_groups, weight_scale=spec.weight_scale, correction=self.correction,
+                               renormalize=spec.renormalize, identity=spec.identity, weight_input=spec.weight_input, shared=self.shared,
+                               shared_gated=_gated(spec.shared), shared_gate=bool(spec.shared_gate))
 
     @staticmethod
     def _router_key(spec):
@@ -262,7 +300,7 @@ class ScoreRoutedExperts(FeedForward):
 
     def forward_terms(self, y, ctx):
         s = self.spec
-        if not s.weight_input or s.shared is not None:
+        if not s.weight_input or s.shared is not None or (self.few is not None and y.shape[0] <= kernels.MOE_TOKENS):
             return super().forward_terms(y, ctx)
         out, pair_row = self._experts(y, *self._route(y)[:2])
         return {"a": out, "pair_row": pair_row}
@@ -276,6 +314,8 @@ class ScoreRoutedExperts(FeedForward):
 
     def forward(self, y, residual, ctx):
         s, rt = self.spec, self.runtime
+        if self.few is not None and y.shape[0] <= kernels.MOE_TOKENS:
+            return kernels.moe_tokens(self.few, y, residual, out=residual)
         chosen, pair_weight, shared_gate = self._route(y)
         if self.shared is not None:
             hidden = kernels.gated_unit(linear(rt, y, self.shared[0]), s.shared.limit, s.shared.alpha, form=s.shared.activation,

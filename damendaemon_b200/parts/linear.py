@@ -69,7 +69,9 @@ def linear(runtime, a, w, bias=None, residual=None, activation=None, out_dtype=N
     beyond 128, see splits_float32); for small matrices and rows that are not 16-byte aligned, or if the runtime asks for 'simt',
     the CUDA-core float32 kernel, whose rows do not depend on what is beside them.
     bfloat16 engine: the tcgen05 tensor-core kernel, unless the runtime asks for 'simt' or the
-    reduction width is no multiple of 8 (then the CUDA-core kernel with bfloat16 operands)."""
+    reduction width is no multiple of 8 (then the CUDA-core kernel with bfloat16 operands). A 4-bit matrix has its own product."""
+    if isinstance(w, kernels.Mx4Matrix):
+        return kernels.gemm_mx4(a, w, bias, residual, activation, out_dtype, out)
     if a.dtype == torch.float32 and runtime.gemm != "simt" and out_dtype in (None, torch.float32) and \
             splits_float32(w.shape[0], a.shape[1]) and kernels.gemm_split_fits(a, w):
         if streams_float32(a.shape[0], w.shape[0], a.shape[1]):
@@ -102,6 +104,8 @@ def grouped_tile(tensor_cores, pairs, groups):
 def grouped_linear(tensor_cores, a, w, tile_group, tile, out_dtype=None, activation=None, row_scale=None):
     """Rows of a in tiles of ``tile``; tile i is multiplied with w[tile_group[i]] (w: [groups, out, in]); tiles whose
     group is negative are skipped. act(row_scale[r] * product), row_scale float32 [rows] or None, in the product's epilogue."""
+    if isinstance(w, kernels.Mx4Matrix):
+        return kernels.gemm_grouped_mx4(a, w, tile_group, tile, out_dtype=out_dtype, activation=activation, row_scale=row_scale)
     if tensor_cores:
         return kernels.gemm_grouped_tcgen05(a, w, tile_group, tile, out_dtype=out_dtype or a.dtype, activation=activation, row_scale=row_scale)
     return kernels.gemm_simt_grouped(a, w, tile_group, activation=activation, out_dtype=out_dtype or a.dtype, row_scale=row_scale)
@@ -111,6 +115,8 @@ def grouped_gated_unit(tensor_cores, a, gate_up, tile_group, tile, limit, alpha,
     """The gated unit (form: one of kernels.GATED_FORMS) over grouped rows: gate_up [groups, 2 * inner, in] holds a group's
     gate rows, then its up rows. On the tensor cores both products and the unit are one kernel; else a grouped product and
     the unit's own kernel."""
+    if isinstance(gate_up, kernels.Mx4Matrix):
+        return kernels.gemm_grouped_mx4(a, gate_up, tile_group, tile, gated=(limit, alpha, form))
     if tensor_cores:
         return kernels.gemm_grouped_tcgen05(a, gate_up, tile_group, tile, gated=(limit, alpha, form))
     return kernels.gated_unit(kernels.gemm_simt_grouped(a, gate_up, tile_group), limit, alpha, form=form)

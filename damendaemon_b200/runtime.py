@@ -18,18 +18,19 @@ from .text_stream import TextStream, checked_stops
 class Runtime:
     def __init__(self, model, context=None, *, dtype="bfloat16", kv_cache_tokens=None, max_batch=16, page_size=16,
                  device="cuda:0", use_graph=True, prefill_chunk_size=0, token_budget=4096, config=None, tensors=None,
-                 run_ahead=True, queue_timeout=None):
+                 run_ahead=True, queue_timeout=None, feed_forward="auto"):
         """model: a folder with config.json and model.safetensors (or None with config= and tensors=).
         context: most tokens a request may hold (default: the model's positions).
         kv_cache_tokens: size of the shared page pool in tokens (default: max_batch * context).
         prefill_chunk_size: largest prompt portion per step, 0 = up to the token budget.
         run_ahead: launch the next decode step before this step's tokens are read (see the scheduler).
-        queue_timeout: seconds a request may wait for cache pages before it fails (None: no limit)."""
+        queue_timeout: seconds a request may wait for cache pages before it fails (None: no limit).
+        feed_forward: 'mx4' holds the feed-forwards' matrices in microscaled 4-bit numbers (see Engine)."""
         positions = _positions(model, config, tensors) or context or Engine.UNBOUNDED_CONTEXT   # a model may name no limit
         self.engine = Engine(model, config=config, tensors=tensors, dtype=dtype, page_size=page_size,
                              max_requests=max_batch, device=device,
                              kv_tokens=kv_cache_tokens or max_batch * min(context or 10 ** 9, positions),
-                             check_device_errors=False, use_graph=use_graph, max_context=min(context or positions, positions))
+                             check_device_errors=False, use_graph=use_graph, feed_forward=feed_forward, max_context=min(context or positions, positions))
         self.context = min(context or self.engine.max_context, self.engine.max_context)
         self.prefill_chunk_size = prefill_chunk_size
         self.token_budget = token_budget
@@ -151,9 +152,9 @@ def _load_tokenizer(model):
 
 
 def generate(model, prompts, max_new_tokens=128, *, temperature=0, seed=None, ignore_eos=True, dtype="bfloat16",
-             page_size=16, kv_tokens=None, **options):
+             page_size=16, kv_tokens=None, feed_forward="auto", **options):
     """One call from a model folder to new token ids: ``generate(dir, [[ids], ...], 16)``."""
     runtime = Runtime(model, dtype=dtype, page_size=page_size, kv_cache_tokens=kv_tokens,
-                      max_batch=max(1, min(64, len(prompts))))
+                      max_batch=max(1, min(64, len(prompts))), feed_forward=feed_forward)
     return runtime.generate_batch(prompts, max_new_tokens, ignore_eos=ignore_eos, temperature=temperature, seed=seed,
                                   **options)
