@@ -14,6 +14,11 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // Eight bfloat16 values of a row from element k on, zeros from element n on; wide: the row is whole 16-byte pieces. (The element by
 // element form is a call: inlined, it would lie between the instructions of every user.)
 static __device__ __noinline__ uint4 load8_slow(const __nv_bfloat16* row, int k, int n) {

@@ -40,7 +40,7 @@ struct DdExpertLayer {
 };
 
 namespace {
-constexpr int UP_THREADS = 512, UP_WARPS = 16, TERMS = 3, SHARE_WIN = 12, MAX_TOKENS = 8, MAX_TOP = 16, MAX_UNITS = MAX_TOKENS * MAX_TOP, MAX_OUTPUTS = 256;
+constexpr int UP_THREADS = 512, UP_WARPS = 16, TERMS = 3, MAX_TOKENS = 8, MAX_TOP = 16, MAX_UNITS = MAX_TOKENS * MAX_TOP, MAX_OUTPUTS = 256;
 enum Kind { F32 = 0, BF16 = 1, MX4 = 2 };
 
 // What up_kernel tells down_kernel.
@@ -63,6 +63,7 @@ struct Call {
     int T, ldy, ldr, ldo, max_units;
     int row, shared_row;         // elements of a hidden row: whole steps, zeros behind the last feature
     int y_wide, router_wide, w_wide, inner_wide;        // rows of whole 16-byte pieces (w: all matrices that meet y, inner: all down)
+    int router_tiles, share_shift, cluster_shift;                    // of the routing: rows by 16, warps and blocks that share columns (log2)
     int cluster, y_pitch, stages;                                    // y_pitch: bytes of a token's row in up_kernel's shared memory
 };
 struct Maps { CUtensorMap gate_up, shared_gate_up, down, shared_down; };
@@ -70,16 +71,19 @@ struct Maps { CUtensorMap gate_up, shared_gate_up, down, shared_down; };
 struct Tile { float sum[16][few::COLUMNS + 1]; };
 template <int N> struct Count { static constexpr int value = N; };
 
-// What a warp multiplies at a time, a tile: 16 rows of a matrix on mma.sync, 4 with multiply-adds, as two boxes of half of them.
+// What a warp multiplies at a time, a tile: 16 rows of a matrix on mma.sync, 4 with multiply-adds. A stage of its ring is one TMA box
+// of a tile (two boxes of half the rows, or half the columns, took 4-bit matrices at 2 TB/s: a copy costs about 50 clocks
+// whatever its size).
 template <int KIND> struct Stream {
     static constexpr int ROWS = KIND == F32 ? few::F32_ROWS : 16, HALF = ROWS / 2;
-    static constexpr int STEP = KIND == BF16 ? 64 : 128;             // k
-    static constexpr int BOX_WIDTH = KIND == MX4 ? mx4::GROUP_BYTES : STEP, BOX_ROW = KIND == F32 ? 512 : KIND == BF16 ? 128 : 64;   // elements, bytes
-    static constexpr int BOX_BYTES = HALF * BOX_ROW, STAGE_BYTES = 2 * BOX_BYTES;
+    static constexpr int STEP = KIND == BF16 ? 64 : KIND == F32 ? 128 : 256;         // k
+    static constexpr int SUB = KIND == MX4 ? 2 : 1;                                  // groups of 128 in it
+    static constexpr int BOX_ROW = KIND == F32 ? 512 : 128, STAGE_BYTES = ROWS * BOX_ROW;
+    static constexpr int BOX_WIDTH = KIND == MX4 ? 128 : STEP;                       // elements as TMA counts them
     static constexpr int ELEMENT = KIND == F32 ? 4 : 2;
-    static constexpr int MOST_STAGES = 8192 / STAGE_BYTES;
+    static constexpr int MOST_STAGES = 4;
 };
-__host__ __device__ constexpr int step_of(int kind) { return kind == BF16 ? 64 : 128; }
+__host__ __device__ constexpr int step_of(int kind) { return kind == BF16 ? 64 : kind == F32 ? 128 : 256; }
 
 // The boxes of a stage without TMA (rows that are no whole 16-byte pieces), in the layout that TMA gives them.
 template <int KIND>
@@ -108,12 +112,10 @@ template <int KIND> struct Ring {
     int stages, asked = 0, taken = 0;            // stage numbers; their phase follows from how often they wrapped
     uint32_t phase = 0;
     __device__ __forceinline__ Ring(uint64_t* b, uint32_t at, int n) : bars(b), base(at), stages(n) {}
-    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row_a, int row_b) {
+    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row, int matrix) {
         uint64_t* bar = &bars[asked];
-        uint8_t* slot = reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES));
         tc::mbar_expect_tx(bar, S::STAGE_BYTES);
-        tc::tma_load_2d(slot, map, step * S::BOX_WIDTH, row_a, bar);
-        tc::tma_load_2d(slot + S::BOX_BYTES, map, step * S::BOX_WIDTH, row_b, bar);
+        tc::tma_load_3d(reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES)), map, step * S::BOX_WIDTH, row, matrix, bar);
     }
     __device__ __forceinline__ void next_asked() { asked = asked + 1 == stages ? 0 : asked + 1; }
     // the address of the next stage to read; `here`: it has been asked for
@@ -125,35 +127,63 @@ template <int KIND> struct Ring {
     }
 };
 
-// 16-byte pieces of a step's other operand that a lane reads for one column, and where: on mma.sync lane (g, t) takes for row g
-// and g + 8 of the matrix the pieces 2 t and 2 t + 1 of 64 bfloat16 numbers (under TMA's 128-byte swizzle eight lanes then meet in
-// no bank), or the t-th eighth of every block of a 4-bit group.
+// What a warp multiplies without a pause: 64 k of a bfloat16 matrix, a group of 128 of a 4-bit one. 16-byte pieces of the other operand
+// that a lane reads for one column, and where: on mma.sync lane (g, t) takes for row g and g + 8 of the matrix the pieces 2 t and
+// 2 t + 1 of 64 bfloat16 numbers (under TMA's 128-byte swizzle eight lanes then meet in no bank), or the t-th eighth of every block of a
+// 4-bit group.
 template <int KIND> constexpr int PIECES = KIND == MX4 ? 4 : 2;
+template <int KIND> constexpr int PART = KIND == MX4 ? 128 : 64;
 template <int KIND>
-__device__ __forceinline__ void take_column(uint4* b, const __nv_bfloat16* x, int step) {
+__device__ __forceinline__ void take_column(uint4* b, const __nv_bfloat16* x, int part) {
     const int t = threadIdx.x & 3;
-    const uint4* from = reinterpret_cast<const uint4*>(x + step * Stream<KIND>::STEP);
+    const uint4* from = reinterpret_cast<const uint4*>(x + part * PART<KIND>);
 #pragma unroll
     for (int i = 0; i < PIECES<KIND>; ++i) b[i] = from[KIND == MX4 ? 4 * i + t : 2 * t + i];
 }
-// A step of a tile by P times eight columns. four0, four1: the scales of a 4-bit group of rows g and g + 8.
-template <int KIND, int P>
-__device__ __forceinline__ void mma_step(uint32_t slot, uint32_t four0, uint32_t four1, const uint4 (*b)[PIECES<KIND>], float (*d)[4]) {
+// The scales of sixteen 4-bit groups of rows g and g + 8: lane (g, t) holds those of groups 4 t .. 4 t + 3, and asks for them a
+// stretch of sixteen ahead (a lane's four bytes a step, requested one step ahead, came from L2 or beyond at every step: 1 us).
+struct Scales {
+    static constexpr int STRETCH = 16;
+    uint32_t a[4], b[4];
+    __device__ __forceinline__ void load(const uint32_t* rows, size_t row_a, size_t row_b, size_t last, int groups, int from, int to) {
+        const int lane = threadIdx.x & 31, first = from + (lane & 3) * 4;
+        const uint32_t *p = rows + min(row_a + (lane >> 2), last) * groups, *q = rows + min(row_b + (lane >> 2), last) * groups;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = first + j < to ? p[first + j] : 0u;
+            b[j] = first + j < to ? q[first + j] : 0u;
+        }
+    }
+    // those of group number i of the stretch
+    __device__ __forceinline__ void get(int i, uint32_t& four_a, uint32_t& four_b) const {
+        const int from = (threadIdx.x & 28) | (i >> 2);
+        four_a = __shfl_sync(0xffffffffu, i & 2 ? (i & 1 ? a[3] : a[2]) : (i & 1 ? a[1] : a[0]), from);
+        four_b = __shfl_sync(0xffffffffu, i & 2 ? (i & 1 ? b[3] : b[2]) : (i & 1 ? b[1] : b[0]), from);
+    }
+};
+
+// A part of a tile (its sub-th in the stage) by P times eight columns. four0, four1: the scales of a 4-bit group of rows g and g + 8.
+// F16: the other operand is float16 (in the order of mx4::pairs_f16), not bfloat16.
+template <int KIND, int P, bool F16 = false>
+__device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0, uint32_t four1, const uint4 (*b)[PIECES<KIND>], float (*d)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if constexpr (KIND == MX4) {
-        const uint32_t at = slot + g * 64 + (t ^ (g >> 1 & 3)) * 16;
-        const uint4 a0 = few::lds16(at), a1 = few::lds16(at + Stream<KIND>::BOX_BYTES);
+        const uint32_t at = slot + g * 128 + ((4 * sub + t) ^ g) * 16;
+        const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
         const uint32_t r0[4] = {a0.x, a0.y, a0.z, a0.w}, r1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             uint32_t v0[4], v1[4];
-            mx4::pairs(r0[i], v0);
-            mx4::pairs(r1[i], v1);
+            if (F16) { mx4::pairs_f16(r0[i], v0); mx4::pairs_f16(r1[i], v1); }
+            else { mx4::pairs(r0[i], v0); mx4::pairs(r1[i], v1); }
             const float by0 = mx4::scale(four0, i), by1 = mx4::scale(four1, i);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 float e[4] = {0.f, 0.f, 0.f, 0.f};
-                few::block_product(v0, v1, b[p][i], e);
+                if (F16) {
+                    few::mma_f16(e, v0[0], v1[0], v0[1], v1[1], b[p][i].x, b[p][i].y);
+                    few::mma_f16(e, v0[2], v1[2], v0[3], v1[3], b[p][i].z, b[p][i].w);
+                } else few::block_product(v0, v1, b[p][i], e);
                 few::add_block(by0, by1, e, d[p]);
             }
         }
@@ -161,7 +191,7 @@ __device__ __forceinline__ void mma_step(uint32_t slot, uint32_t four0, uint32_t
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t at = slot + g * 128 + ((2 * t + i) ^ g) * 16;
-            const uint4 a0 = few::lds16(at), a1 = few::lds16(at + Stream<KIND>::BOX_BYTES);
+            const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 few::mma(d[p], a0.x, a1.x, a0.y, a1.y, b[p][i].x, b[p][i].y);
@@ -170,11 +200,10 @@ __device__ __forceinline__ void mma_step(uint32_t slot, uint32_t four0, uint32_t
         }
     }
 }
-template <int KIND>
-__device__ __forceinline__ void put_tile(Tile& to, const float* d) {
+__device__ __forceinline__ void put_tile(Tile& to, const float* d, float by = 1.f) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i] * (KIND == MX4 ? few::MX4_BACK : 1.f);
+    for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i] * by;
 }
 
 // Up to eight token numbers, ascending, four bits each.
@@ -234,6 +263,8 @@ struct Routing {
     int chosen[MAX_TOKENS][MAX_TOP];
     float weight[MAX_TOKENS][MAX_TOP];
     float gate[MAX_TOKENS];                      // the shared unit's
+    uint32_t y_top[MAX_TOKENS];                  // bits of a token's largest |y| (4-bit matrices)
+    float y_back[MAX_TOKENS];                    // what its float16 row has to be multiplied with
     uint32_t users[MAX_OUTPUTS];                 // per output: which tokens chose it
     int count[UP_WARPS];
     int n_units;
@@ -247,12 +278,12 @@ struct Routing {
 struct RouterItem {
     int tile, from, to;
     __device__ __forceinline__ RouterItem(const Call& c, int kind, int item) {
-        const int rows = c.l.experts + c.l.identity + c.l.shared_gate, tiles = (rows + 15) / 16, shares = max(1, UP_WARPS / tiles);
-        const int steps = (c.l.width + (kind == F32 ? 127 : 31)) / (kind == F32 ? 128 : 32), rank = c.cluster > 1 ? (int)tc::cluster_rank() : 0;
-        const int begin = steps * rank / c.cluster, end = steps * (rank + 1) / c.cluster, share = item / tiles;
-        tile = item % tiles;
-        from = begin + (end - begin) * share / shares;
-        to = begin + (end - begin) * (share + 1) / shares;
+        const int steps = (c.l.width + (kind == F32 ? 127 : 31)) / (kind == F32 ? 128 : 32), rank = c.cluster_shift ? (int)tc::cluster_rank() : 0;
+        const int begin = steps * rank >> c.cluster_shift, end = steps * (rank + 1) >> c.cluster_shift;
+        int share = 0;
+        for (tile = item; tile >= c.router_tiles; tile -= c.router_tiles) ++share;
+        from = begin + ((end - begin) * share >> c.share_shift);
+        to = begin + ((end - begin) * (share + 1) >> c.share_shift);
     }
 };
 __device__ __forceinline__ const __nv_bfloat16* router_row(const Call& c, int tile, int i) {
@@ -284,7 +315,7 @@ __device__ void partial_logits(const Call& c, const uint8_t* y, int items, Tile*
             if (item != warp) ahead.load(w0, w1, c.l.width, it.from, it.to, c.router_wide);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             few::stream_bf16(w0, w1, x, c.l.width, it.from, it.to, c.router_wide, ahead, d);
-            put_tile<BF16>(parts[item], d);
+            put_tile(parts[item], d);
         }
     }
 }
@@ -295,7 +326,7 @@ __device__ void route(const Call& c, const uint8_t* y, Routing& r, float* scratc
     const int outputs = c.l.experts + c.l.identity;
     if (threadIdx.x < MAX_OUTPUTS) r.users[threadIdx.x] = 0;
     if (c.l.router) {
-        const int rows = outputs + c.l.shared_gate, tiles = (rows + 15) / 16, shares = max(1, UP_WARPS / tiles);
+        const int rows = outputs + c.l.shared_gate, tiles = c.router_tiles, shares = 1 << c.share_shift;
         const int n = tiles * 16 * MAX_TOKENS;                          // logits, a row of eight an output
         const int rank = c.cluster > 1 ? (int)tc::cluster_rank() : 0;
         Tile* parts = reinterpret_cast<Tile*>(scratch);
@@ -333,7 +364,10 @@ __device__ void route(const Call& c, const uint8_t* y, Routing& r, float* scratc
         __syncthreads();
         if (warp < c.T) {
             float *sc = score + warp * outputs, *v = value + warp * outputs, *wo = worth + warp * max(c.l.groups, MAX_TOP);
-            if (outputs <= 64)
+            if (outputs <= 32)
+                dd_choose_few<1>(sc, v, wo, outputs, c.l.top, c.l.groups, c.l.keep, c.l.weight_scale, c.l.softmax, c.l.correction, c.l.renormalize,
+                                 r.chosen[warp], r.weight[warp]);
+            else if (outputs <= 64)
                 dd_choose_few<2>(sc, v, wo, outputs, c.l.top, c.l.groups, c.l.keep, c.l.weight_scale, c.l.softmax, c.l.correction, c.l.renormalize,
                                  r.chosen[warp], r.weight[warp]);
             else
@@ -453,6 +487,8 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     }
     bars.init();
     if (threadIdx.x == 0) {
+        if (c.w_wide) tc::prefetch_tensormap(&maps.gate_up);
+        if (c.w_wide && c.l.shared_inner) tc::prefetch_tensormap(&maps.shared_gate_up);
         tc::mbar_init(&r.arrived, 1);
         tc::fence_barrier_init();
     }
@@ -479,7 +515,47 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             }
     }
     __syncthreads();
-    route<KIND>(c, y, r, reinterpret_cast<float*>(y + c.T * c.y_pitch), ahead, &bars.gave_up);
+    // 4-bit matrices meet the rows as float16 (their elements become that in one instruction): times a power of two that brings a
+    // row's largest element to 2^14, every bfloat16 of more than 2^-31 of it is kept exactly, what is below to 2^-39 of it
+    uint8_t* x_rows = y;
+    if constexpr (KIND == MX4) {
+        x_rows = y + c.T * c.y_pitch;
+        const int pieces = (c.y_pitch - 16) / 16, by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;
+        if (threadIdx.x < MAX_TOKENS) r.y_top[threadIdx.x] = 0;
+        __syncthreads();
+        if (t < c.T) {
+            uint32_t top = 0;
+#pragma unroll 1
+            for (int at = (warp % by) * 32 + lane; at < pieces; at += by * 32) {
+                const uint4 v = *reinterpret_cast<const uint4*>(y + t * c.y_pitch + at * 16);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = max(top, max(w[i] << 16 & 0x7fff0000u, w[i] & 0x7fff0000u));
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(&r.y_top[t], top);
+        }
+        __syncthreads();
+        if (t < c.T) {
+            const int exponent = (int)(r.y_top[t] >> 23), up = exponent == 255 ? 0 : min(126, 141 - exponent);      // times 2^up
+            const float times = __uint_as_float((uint32_t)(up + 127) << 23);
+            if (warp % by == 0 && lane == 0) r.y_back[t] = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll 1
+            for (int at = (warp % by) * 32 + lane; at < pieces; at += by * 32) {
+                const uint4 v = *reinterpret_cast<const uint4*>(y + t * c.y_pitch + at * 16);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t even[2], odd[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(even[i]) : "f"(__uint_as_float(w[2 * i + 1] << 16) * times), "f"(__uint_as_float(w[2 * i] << 16) * times));
+                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(odd[i]) : "f"(__uint_as_float(w[2 * i + 1] & 0xffff0000u) * times),
+                        "f"(__uint_as_float(w[2 * i] & 0xffff0000u) * times));
+                }
+                *reinterpret_cast<uint4*>(x_rows + t * c.y_pitch + at * 16) = make_uint4(even[0], even[1], odd[0], odd[1]);
+            }
+        }
+    }
+    route<KIND>(c, y, r, reinterpret_cast<float*>(x_rows + c.T * c.y_pitch), ahead, &bars.gave_up);
     if (blockIdx.x == 0) {
         for (int u = threadIdx.x; u < r.n_units; u += UP_THREADS) {
             c.plan->expert[u] = r.expert[u];
@@ -498,27 +574,26 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     const int features = c.l.gated ? S::HALF : S::ROWS;
     const int per_unit = (c.l.inner + features - 1) / features, for_shared = (c.l.shared_inner + S::HALF - 1) / S::HALF;
     const int total = for_shared + r.n_units * per_unit;
-    // `share` warps share a tile's columns: what leaves the fewest warps idle in the last round (the tiles are dealt out over the
-    // blocks first). A tile alone in a warp needs no barrier of the block, so sharers have to win a quarter of the time.
+    const float per_unit_inverse = 1.0f / (float)per_unit;
+    // `share` warps share a tile's columns: as few as give most warps a tile (with more tiles than warps the last round's are spread
+    // over the SMs, and enough of them to keep the memory busy; a tile alone in a warp needs no barrier of the block)
     const int warps = gridDim.x * UP_WARPS;
     int share = 1;
-#pragma unroll 1
-    for (int s = 2, best = (total + warps - 1) / warps * 16; s <= UP_WARPS; s *= 2) {
-        const int cost = (total * s + warps - 1) / warps * 16 / s;
-        if (cost < best * SHARE_WIN / 16) { best = cost; share = s; }
-    }
+    while (share < UP_WARPS && total * share * 4 < warps * 3) share *= 2;
     const int slots = UP_WARPS / share, slot = warp / share, part = warp % share, stride = gridDim.x * slots;
     const int steps = (width + S::STEP - 1) / S::STEP, from = steps * part / share, to = steps * (part + 1) / share;
-    // a tile: its unit (-1: the shared one), first feature, and the rows of the matrix where its two boxes begin: gate rows and the same
-    // features' up rows; plain: neighbours
-    struct Place { int unit, first, row_a, row_b; };
+    // a tile: its unit (-1: the shared one), first feature, matrix of the stack (gate and up are two), and the rows where its halves begin:
+    // gate rows and the same features' up rows; plain: neighbours
+    struct Place { int unit, first, matrix, row_a, row_b; };
     auto place_of = [&](int tile) {
         Place p;
-        p.unit = tile < for_shared ? -1 : (tile - for_shared) / per_unit;
+        // (a float's quotient of whole numbers below 2^21, half a step off the border, is on the right side of it)
+        p.unit = tile < for_shared ? -1 : (int)(((float)(tile - for_shared) + 0.5f) * per_unit_inverse);
         const bool gated = p.unit < 0 || c.l.gated;
         const int inner = p.unit < 0 ? c.l.shared_inner : c.l.inner;
         p.first = p.unit < 0 ? tile * S::HALF : (tile - for_shared - p.unit * per_unit) * features;
-        p.row_a = (p.unit < 0 ? 0 : r.expert[p.unit] * inner * (gated ? 2 : 1)) + p.first;
+        p.matrix = p.unit < 0 ? 0 : r.expert[p.unit] * (gated ? 2 : 1);
+        p.row_a = p.matrix * inner + p.first;
         p.row_b = p.row_a + (gated ? inner : S::HALF);
         return p;
     };
@@ -529,7 +604,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     if (f_tile < total) f = place_of(f_tile);
     auto fetch = [&] {
         if (f_tile >= total || from >= to) return;
-        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.row_a, f.row_b);
+        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.first, f.matrix);
         ring.next_asked();
         if (++f_step == to) {
             f_step = from;
@@ -539,8 +614,18 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     };
 #pragma unroll 1
     for (int i = 0; i < c.stages - 1; ++i) fetch();
+    Scales have, soon;
+    const int groups = (width + mx4::GROUP - 1) / mx4::GROUP;
+    auto ask_scales = [&](int tile, int at) {
+        const Place p = place_of(tile);
+        const bool shared = p.unit < 0;
+        soon.load(reinterpret_cast<const uint32_t*>(shared ? c.l.shared_gate_up_scales : c.l.gate_up_scales), p.row_a, p.row_b,
+                  (shared ? (size_t)2 * c.l.shared_inner : (size_t)c.l.experts * c.l.inner * (c.l.gated ? 2 : 1)) - 1, groups, at * S::SUB,
+                  min(to * S::SUB, groups));
+    };
+    if (KIND == MX4 && slot * gridDim.x + blockIdx.x < total && from < to) ask_scales(slot * gridDim.x + blockIdx.x, from);
     // (columns beyond the tokens read the last one's row; nobody looks at them)
-    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(y + min(lane >> 2, c.T - 1) * c.y_pitch);
+    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(x_rows + min(lane >> 2, c.T - 1) * c.y_pitch);
     // (with shared tiles every warp of the block takes part in every round's barrier)
     for (int turn = 0, round = blockIdx.x; round < total; round += stride, turn ^= 1) {
         const int tile = round + slot * gridDim.x;
@@ -587,28 +672,30 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
         } else {
             float d[1][4] = {};
             if (mine) {
-                const uint32_t *s0 = nullptr, *s1 = nullptr;
-                uint32_t four0 = 0, four1 = 0;
-                if (KIND == MX4) {
-                    const size_t groups = steps, last = matrix_rows - 1;
-                    const uint32_t* scales = reinterpret_cast<const uint32_t*>(shared ? c.l.shared_gate_up_scales : c.l.gate_up_scales);
-                    s0 = scales + min((size_t)p.row_a + (lane >> 2), last) * groups;
-                    s1 = scales + min((size_t)p.row_b + (lane >> 2), last) * groups;
-                    if (from < to) { four0 = s0[from]; four1 = s1[from]; }
-                }
                 for (int s = from; s < to; ++s) {
-                    uint4 b[1][PIECES<KIND>];
-                    take_column<KIND>(b[0], x, s);
-                    uint32_t n0 = 0, n1 = 0;
-                    if (KIND == MX4 && s + 1 < to) { n0 = s0[s + 1]; n1 = s1[s + 1]; }
-                    mma_step<KIND, 1>(next(s), four0, four1, b, d);
-                    four0 = n0; four1 = n1;
+                    const uint32_t at = next(s);
+#pragma unroll
+                    for (int sub = 0; sub < S::SUB; ++sub) {
+                        uint32_t four0 = 0, four1 = 0;
+                        if (KIND == MX4) {
+                            const int i = ((s - from) * S::SUB + sub) % Scales::STRETCH, then = s + Scales::STRETCH / S::SUB;
+                            if (i == 0) {         // this stretch's have come; the next one's, of this tile or the warp's next, are asked for
+                                have = soon;
+                                if (then < to) ask_scales(tile, then);
+                                else if (tile + stride < total) ask_scales(tile + stride, from);
+                            }
+                            have.get(i, four0, four1);
+                        }
+                        uint4 b[1][PIECES<KIND>];
+                        take_column<KIND>(b[0], x, s * S::SUB + sub);
+                        mma_step<KIND, 1, KIND == MX4>(at, sub, four0, four1, b, d);
+                    }
                     __syncwarp();
                     fetch();
                 }
             }
             if (share > 1) {                      // the first of the sharers adds up
-                put_tile<KIND>(red[turn][warp], d[0]);
+                put_tile(red[turn][warp], d[0]);
                 __syncthreads();
                 if (mine && part == 0) {
                     const int g = lane >> 2, t = lane & 3;
@@ -619,9 +706,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                         d[0][i] = sum;
                     }
                 }
-            } else if (KIND == MX4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[0][i] *= few::MX4_BACK;
+            }
             if (mine && part == 0) {
                 // lane (g, t): features g (and g + 8 of a plain unit) of tokens 2 t and 2 t + 1
                 const int inner = shared ? c.l.shared_inner : c.l.inner, g = lane >> 2;
@@ -630,7 +715,8 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 for (int i = 0; i < 4; ++i) {
                     const int t = 2 * (lane & 3) + (i & 1), feature = p.first + g + (i >> 1) * S::HALF;
                     if ((gated && i > 1) || feature >= inner || !(users >> t & 1)) continue;
-                    put_hidden<KIND>(c, shared, p.unit, t, feature, unit_value(c, shared, d[0][i], d[0][i | 2], shared ? r.gate[t] : r.unit_weight[p.unit][t]));
+                    const float back = KIND == MX4 ? r.y_back[t] : 1.f;
+                    put_hidden<KIND>(c, shared, p.unit, t, feature, unit_value(c, shared, d[0][i] * back, d[0][i | 2] * back, shared ? r.gate[t] : r.unit_weight[p.unit][t]));
                 }
             }
         }
@@ -657,6 +743,10 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     dd_launch_dependents();
     if (c.l.shared_inner && c.inner_wide) ask_for(c.l.shared_down, matrix_bytes(KIND, c.l.width, c.l.shared_inner));
     bars.init();
+    if (threadIdx.x == 0 && c.inner_wide) {
+        tc::prefetch_tensormap(&maps.down);
+        if (c.l.shared_inner) tc::prefetch_tensormap(&maps.shared_down);
+    }
     for (int i = lane; i < (int)(sizeof(Tile) / 4); i += 32) reinterpret_cast<float*>(&red[warp])[i] = 0.f;
     dd_grid_wait();
     // (all of it at once, used or not)
@@ -679,9 +769,9 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     // step -> unit (-1: the shared one), its first step and its end
     auto unit_of = [&](int at) { return at < for_shared ? -1 : (at - for_shared) / per_unit; };
     auto begin_of = [&](int unit) { return unit < 0 ? 0 : for_shared + unit * per_unit; };
-    auto row_of = [&](int unit) { return (unit < 0 ? 0 : plan.expert[unit] * c.l.width) + n0; };
+    auto matrix_of = [&](int unit) { return unit < 0 ? 0 : plan.expert[unit]; };
     Ring<KIND> ring(bars.full[warp], tc::smem_u32(smem) + warp * STAGES * S::STAGE_BYTES, STAGES);
-    int f_at = from, f_begin = 0, f_end = from, f_row = 0;
+    int f_at = from, f_begin = 0, f_end = from, f_matrix = 0;
     bool f_shared = false;
     auto fetch = [&] {
         if (f_at >= to) return;
@@ -690,15 +780,24 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             f_shared = unit < 0;
             f_begin = begin_of(unit);
             f_end = begin_of(unit + 1);
-            f_row = row_of(unit);
+            f_matrix = matrix_of(unit);
         }
         if (c.inner_wide && lane == 0)
-            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, f_row, f_row + S::HALF);
+            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, n0, f_matrix);
         ring.next_asked();
         ++f_at;
     };
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) fetch();
+    Scales have, soon;
+    auto ask_scales = [&](int unit, int at) {     // of a unit, from step `at` on
+        const bool shared = unit < 0;
+        const int begin = begin_of(unit);
+        const int row = matrix_of(unit) * c.l.width + n0, groups = ((shared ? c.l.shared_inner : c.l.inner) + mx4::GROUP - 1) / mx4::GROUP;
+        soon.load(reinterpret_cast<const uint32_t*>(shared ? c.l.shared_down_scales : c.l.down_scales), row, row + S::HALF,
+                  (size_t)(shared ? 1 : c.l.experts) * c.l.width - 1, groups, (at - begin) * S::SUB, min((min(to, begin_of(unit + 1)) - begin) * S::SUB, groups));
+    };
+    if (KIND == MX4 && from < to) ask_scales(unit_of(from), from);
     for (int at = from; at < to;) {               // the runs of steps of one unit
         const int unit = unit_of(at), begin = begin_of(unit), end = min(to, begin_of(unit + 1));
         const bool shared = unit < 0;
@@ -707,7 +806,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
         const int n = __popc(users);
         const size_t hidden = (size_t)(shared ? c.max_units : unit) * c.T * c.row, matrix_rows = (size_t)(shared ? 1 : c.l.experts) * c.l.width;
         const void* matrix = shared ? c.l.shared_down : c.l.down;
-        const int first_row = row_of(unit);
+        const int first_row = matrix_of(unit) * c.l.width + n0;
         auto next = [&](int s) {
             const uint32_t place = ring.take(c.inner_wide, &bars.gave_up);
             if (!c.inner_wide) fill_stage<KIND>(place, matrix, first_row, first_row + S::HALF, matrix_rows, K, s - begin);
@@ -737,41 +836,44 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                     const int q = p * few::COLUMNS + g < n * TERMS ? p * few::COLUMNS + g : 0;
                     x[p] = h + (size_t)(listed(list, q / TERMS) * TERMS + q % TERMS) * ld;
                 }
-                const uint32_t *s0 = nullptr, *s1 = nullptr;
-                uint32_t four0 = 0, four1 = 0;
-                if (KIND == MX4) {
-                    const size_t groups = steps_of(K), last = matrix_rows - 1;
-                    const uint32_t* scales = reinterpret_cast<const uint32_t*>(shared ? c.l.shared_down_scales : c.l.down_scales);
-                    s0 = scales + min((size_t)first_row + g, last) * groups;
-                    s1 = scales + min((size_t)first_row + g + 8, last) * groups;
-                    four0 = s0[at - begin]; four1 = s1[at - begin];
-                }
-                // a step's columns and scales are requested a step ahead where there are registers for it
-                constexpr int AHEAD = P * Q <= 4 ? 1 : 0;
+                // a part's columns are requested some parts ahead, as far as there are registers for it
+                constexpr int AHEAD = P == 1 ? (KIND == BF16 ? 3 : 1) : KIND == BF16 && P == 2 ? 1 : 0, UN = AHEAD + 1 > S::SUB ? AHEAD + 1 : S::SUB;
+                const int first = (at - begin) * S::SUB, parts = (end - at) * S::SUB;
                 uint4 b[AHEAD + 1][P][Q];
-                if (AHEAD)
 #pragma unroll
-                    for (int p = 0; p < P; ++p) take_column<KIND>(b[0][p], x[p], at - begin);
-                for (int s = at; s < end; s += AHEAD + 1)
+                for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-                    for (int u = 0; u <= AHEAD; ++u) {
-                        if (s + u >= end) break;
-                        const int soon = s + u + AHEAD - begin, v = (u + AHEAD) & AHEAD;
-                        if (s + u + AHEAD < end) {
+                    for (int p = 0; p < P; ++p) take_column<KIND>(b[u][p], x[p], first + min(u, parts - 1));
+                uint32_t place = 0;
+                for (int q = 0; q < parts; q += UN)
 #pragma unroll
-                            for (int p = 0; p < P; ++p) take_column<KIND>(b[v][p], x[p], soon);
+                    for (int u = 0; u < UN; ++u) {
+                        if (q + u >= parts) break;
+                        if (u % S::SUB == 0) place = next(at + (q + u) / S::SUB);
+                        if (q + u + AHEAD < parts) {
+#pragma unroll
+                            for (int p = 0; p < P; ++p) take_column<KIND>(b[(u + AHEAD) % (AHEAD + 1)][p], x[p], first + q + u + AHEAD);
                         }
-                        uint32_t n0 = 0, n1 = 0;
-                        if (KIND == MX4 && s + u + 1 < end) { n0 = s0[s + u + 1 - begin]; n1 = s1[s + u + 1 - begin]; }
-                        mma_step<KIND, P>(next(s + u), four0, four1, b[u], d);
-                        four0 = n0; four1 = n1;
-                        __syncwarp();
-                        fetch();
+                        uint32_t four0 = 0, four1 = 0;
+                        if (KIND == MX4) {
+                            const int i = (q + u) % Scales::STRETCH, then = at + (q + u + Scales::STRETCH) / S::SUB;
+                            if (i == 0) {         // the next stretch: of this run, or of the next one
+                                have = soon;
+                                if (then < end) ask_scales(unit, then);
+                                else if (end < to) ask_scales(unit + 1, end);
+                            }
+                            have.get(i, four0, four1);
+                        }
+                        mma_step<KIND, P>(place, u % S::SUB, four0, four1, b[u % (AHEAD + 1)], d);
+                        if (u % S::SUB == S::SUB - 1) {
+                            __syncwarp();
+                            fetch();
+                        }
                     }
                 // into the tokens that use the expert (the others are not touched: zero times a weight that is not finite is no zero)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    put_tile<KIND>(columns[warp], d[p]);
+                    put_tile(columns[warp], d[p], KIND == MX4 ? few::MX4_BACK : 1.f);
                     __syncwarp();
                     if (lane < 16)
                         for (int i = 0; i < few::COLUMNS && p * few::COLUMNS + i < n * TERMS; ++i)
@@ -798,9 +900,10 @@ typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A matrix of the layer as TMA boxes of its kind (Stream); one whose rows are no whole 16-byte pieces has none.
+// Matrices of the layer as TMA boxes of their kind (Stream): a stack of `matrices` of rows x K, boxes of box_rows rows out of box_matrices
+// neighbours (a gate's and the up matrix behind it). Rows that are no whole 16-byte pieces have none.
 template <int KIND>
-int layer_map(CUtensorMap* map, const void* base, long long rows, int K) {
+int layer_map(CUtensorMap* map, const void* base, long long matrices, long long rows, int K, int box_matrices) {
     using S = Stream<KIND>;
     const long long row_bytes = KIND == MX4 ? (long long)dd_ceil_div(K, mx4::GROUP) * mx4::GROUP_BYTES : (long long)K * S::ELEMENT;
     if (!base || rows <= 0 || row_bytes % 16 || ((uintptr_t)base & 15)) return 0;
@@ -813,23 +916,24 @@ int layer_map(CUtensorMap* map, const void* base, long long rows, int K) {
             enc = reinterpret_cast<EncodeTiled>(sym);
     }
     if (!enc) return dd_fail("dd_moe_tokens: cuTensorMapEncodeTiled is not available from this driver");
-    cuuint64_t dims[2] = {(cuuint64_t)(KIND == MX4 ? row_bytes : K), (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
-    cuuint32_t box[2] = {(cuuint32_t)S::BOX_WIDTH, (cuuint32_t)S::HALF};
-    cuuint32_t elem[2] = {1, 1};
+    cuuint64_t dims[3] = {(cuuint64_t)(KIND == MX4 ? row_bytes : K), (cuuint64_t)rows, (cuuint64_t)matrices};
+    cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(row_bytes * rows)};
+    cuuint32_t box[3] = {(cuuint32_t)S::BOX_WIDTH, (cuuint32_t)(S::ROWS / box_matrices), (cuuint32_t)box_matrices};
+    cuuint32_t elem[3] = {1, 1, 1};
     const CUresult r = enc(map, KIND == F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KIND == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
-                           2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : KIND == BF16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return dd_fail("dd_moe_tokens: cannot describe a matrix of %lld x %d to TMA (driver error %d)", rows, K, (int)r);
+                           3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return dd_fail("dd_moe_tokens: cannot describe %lld matrices of %lld x %d to TMA (driver error %d)", matrices, rows, K, (int)r);
     return 0;
 }
 template <int KIND>
 int layer_maps(Maps* m, const DdExpertLayer& l) {
-    if (int e = layer_map<KIND>(&m->gate_up, l.gate_up, (long long)l.experts * l.inner * (l.gated ? 2 : 1), l.width)) return e;
-    if (int e = layer_map<KIND>(&m->down, l.down, (long long)l.experts * l.width, l.inner)) return e;
-    if (int e = layer_map<KIND>(&m->shared_gate_up, l.shared_gate_up, 2ll * l.shared_inner, l.width)) return e;
-    return layer_map<KIND>(&m->shared_down, l.shared_down, l.width, l.shared_inner);
+    const int halves = l.gated ? 2 : 1;
+    if (int e = layer_map<KIND>(&m->gate_up, l.gate_up, (long long)l.experts * halves, l.inner, l.width, halves)) return e;
+    if (int e = layer_map<KIND>(&m->down, l.down, l.experts, l.width, l.inner, 1)) return e;
+    if (int e = layer_map<KIND>(&m->shared_gate_up, l.shared_gate_up, 2, l.shared_inner, l.width, 2)) return e;
+    return layer_map<KIND>(&m->shared_down, l.shared_down, 1, l.width, l.shared_inner, 1);
 }
 
 template <int KIND>
@@ -869,13 +973,16 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     // a router of up to 64 KB is read by every block for itself, a larger one shared by a cluster's blocks
     // (128 outputs and more leave no room for what eight blocks send)
     const size_t router_bytes = c.l.router ? (size_t)rows * c.l.width * S::ELEMENT : 0;
-    const int tiles = (rows + 15) / 16, shares = tiles < UP_WARPS ? UP_WARPS / tiles : 1;
+    const int tiles = (rows + 15) / 16, shares = tiles >= 9 ? 1 : tiles >= 5 ? 2 : tiles >= 3 ? 4 : tiles == 2 ? 8 : 16;
     c.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) || tiles > 8 ? 4 : 8;
+    c.router_tiles = tiles;
+    c.share_shift = shares == 16 ? 4 : shares / 2 - (shares == 8);
+    c.cluster_shift = c.cluster == 8 ? 3 : c.cluster / 2;
     const size_t scratch = !c.l.router ? 0 : sizeof(Tile) * tiles * shares + sizeof(float) * (c.cluster * tiles * 16 * MAX_TOKENS +
                                                                                                 MAX_TOKENS * (2 * outputs + (c.l.groups > MAX_TOP ? c.l.groups : MAX_TOP)));
-    c.y_pitch = dd_ceil_div((long long)c.l.width, 128) * 128 * S::ELEMENT + 16;
+    c.y_pitch = dd_ceil_div((long long)c.l.width, S::STEP) * S::STEP * S::ELEMENT + 16;
     constexpr size_t MOST = 227 * 1024 - 32 * 1024;      // less the static part
-    const size_t fixed = scratch + (size_t)c.T * c.y_pitch + 1024, stage = UP_WARPS * S::STAGE_BYTES;
+    const size_t fixed = scratch + (size_t)c.T * c.y_pitch * (KIND == MX4 ? 2 : 1) + 1024, stage = UP_WARPS * S::STAGE_BYTES;
     if (fixed + 2 * stage > MOST)
         return dd_fail("dd_moe_tokens: %d rows of %d elements are more than a block's shared memory holds beside its rings", c.T, c.l.width);
     c.stages = (int)((MOST - fixed) / stage);
@@ -885,7 +992,7 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     const int most = sms >= 148 ? (c.cluster == 1 ? sms : c.cluster == 4 ? 132 : 120) : sms / 2 / c.cluster * c.cluster;
     const int features = c.l.gated ? S::HALF : S::ROWS;
     const long long at_most = (long long)c.max_units * ((c.l.inner + features - 1) / features) + (c.l.shared_inner + S::HALF - 1) / S::HALF;
-    if (at_most * UP_WARPS > INT_MAX || (long long)c.l.experts * c.l.inner * 2 > INT_MAX || (long long)c.l.experts * c.l.width > INT_MAX)
+    if (at_most > (1 << 21) || (long long)c.l.experts * c.l.inner * 2 > INT_MAX || (long long)c.l.experts * c.l.width > INT_MAX)
         return dd_fail("dd_moe_tokens: %d experts of %d x %d are too large", c.l.experts, c.l.inner, c.l.width);
     const int blocks = at_most < most ? (int)((at_most + c.cluster - 1) / c.cluster * c.cluster) : most;
     if (int e = launch_up<KIND>(c, m, blocks, fixed + c.stages * stage, s)) return e;

@@ -180,7 +180,7 @@ __device__ __forceinline__ void dd_choose_few(float* score, float* value, float*
         // an expert's place is the number of better ones: no reduction waits for the one before it
         int place[N] = {};
 #pragma unroll 4
-        for (int from = 0; from < 32; ++from)
+        for (int from = 0; from < min(32, n_experts); ++from)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const uint32_t other = __shfl_sync(0xffffffffu, key[j], from);
