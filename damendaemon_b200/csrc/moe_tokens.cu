@@ -79,7 +79,6 @@ template <int KIND> struct Stream {
     static constexpr int STEP = KIND == BF16 ? 64 : KIND == F32 ? 128 : 256;         // k
     static constexpr int SUB = KIND == MX4 ? 2 : 1;                                  // groups of 128 in it
     static constexpr int BOX_ROW = KIND == F32 ? 512 : 128, STAGE_BYTES = ROWS * BOX_ROW;
-    static constexpr int BOX_WIDTH = KIND == MX4 ? 128 : STEP;                       // elements as TMA counts them
     static constexpr int ELEMENT = KIND == F32 ? 4 : 2;
     static constexpr int MOST_STAGES = 4;
 };
@@ -112,10 +111,14 @@ template <int KIND> struct Ring {
     int stages, asked = 0, taken = 0;            // stage numbers; their phase follows from how often they wrapped
     uint32_t phase = 0;
     __device__ __forceinline__ Ring(uint64_t* b, uint32_t at, int n) : bars(b), base(at), stages(n) {}
-    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row, int matrix) {
+    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row, int matrix, bool halves) {
         uint64_t* bar = &bars[asked];
+        uint8_t* slot = reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES));
         tc::mbar_expect_tx(bar, S::STAGE_BYTES);
-        tc::tma_load_3d(reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES)), map, step * S::BOX_WIDTH, row, matrix, bar);
+        if (KIND == MX4) {
+            tc::tma_load_4d(slot, map, 0, row, step * S::SUB, matrix, bar);
+            if (!halves) tc::tma_load_4d(slot + S::STAGE_BYTES / 2, map, 0, row + S::HALF, step * S::SUB, matrix, bar);
+        } else tc::tma_load_3d(slot, map, step * S::STEP, row, matrix, bar);
     }
     __device__ __forceinline__ void next_asked() { asked = asked + 1 == stages ? 0 : asked + 1; }
     // the address of the next stage to read; `here`: it has been asked for
@@ -168,7 +171,7 @@ template <int KIND, int P, bool F16 = false>
 __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0, uint32_t four1, const uint4 (*b)[PIECES<KIND>], float (*d)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if constexpr (KIND == MX4) {
-        const uint32_t at = slot + g * 128 + ((4 * sub + t) ^ g) * 16;
+        const uint32_t at = slot + sub * 512 + g * 64 + (t ^ (g >> 1 & 3)) * 16;      // [half][group][row][64 bytes]
         const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
         const uint32_t r0[4] = {a0.x, a0.y, a0.z, a0.w}, r1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
@@ -497,11 +500,11 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
         tc::cluster_wait();
     }
     dd_grid_wait();
-    // the tokens' rows with zeros behind them; a row starts 16 bytes off the one before it, modulo 128, so that eight lanes' pieces
-    // of two rows meet in no bank
+    // the tokens' rows with zeros behind them; a row starts 16 bytes (4-bit matrices: 64) off the one before it, modulo 128, so that
+    // eight lanes' pieces of two rows meet in no bank
     uint8_t* y = smem + UP_WARPS * c.stages * S::STAGE_BYTES;
     {
-        const int pieces = (c.y_pitch - 16) / 16, in = 16 / S::ELEMENT;
+        const int pieces = c.y_pitch / 128 * 8, in = 16 / S::ELEMENT;
         const int by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;          // warps a token
         if (t < c.T)
 #pragma unroll 1
@@ -520,7 +523,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     uint8_t* x_rows = y;
     if constexpr (KIND == MX4) {
         x_rows = y + c.T * c.y_pitch;
-        const int pieces = (c.y_pitch - 16) / 16, by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;
+        const int pieces = c.y_pitch / 128 * 8, by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;
         if (threadIdx.x < MAX_TOKENS) r.y_top[threadIdx.x] = 0;
         __syncthreads();
         if (t < c.T) {
@@ -604,7 +607,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     if (f_tile < total) f = place_of(f_tile);
     auto fetch = [&] {
         if (f_tile >= total || from >= to) return;
-        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.first, f.matrix);
+        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.first, f.matrix, f.unit < 0 || c.l.gated);
         ring.next_asked();
         if (++f_step == to) {
             f_step = from;
@@ -783,7 +786,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             f_matrix = matrix_of(unit);
         }
         if (c.inner_wide && lane == 0)
-            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, n0, f_matrix);
+            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, n0, f_matrix, false);
         ring.next_asked();
         ++f_at;
     };
@@ -916,14 +919,19 @@ int layer_map(CUtensorMap* map, const void* base, long long matrices, long long 
             enc = reinterpret_cast<EncodeTiled>(sym);
     }
     if (!enc) return dd_fail("dd_moe_tokens: cuTensorMapEncodeTiled is not available from this driver");
-    cuuint64_t dims[3] = {(cuuint64_t)(KIND == MX4 ? row_bytes : K), (cuuint64_t)rows, (cuuint64_t)matrices};
-    cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(row_bytes * rows)};
-    cuuint32_t box[3] = {(cuuint32_t)S::BOX_WIDTH, (cuuint32_t)(S::ROWS / box_matrices), (cuuint32_t)box_matrices};
-    cuuint32_t elem[3] = {1, 1, 1};
+    // k, row, matrix; 4 bits: a group's bytes, row, group, matrix, so that a stage holds one group's rows after the other's (and a row's
+    // 64 bytes under the 64-byte swizzle meet in no bank), half the rows of a tile a box
+    constexpr bool FOUR = KIND == MX4;
+    cuuint64_t dims[4] = {(cuuint64_t)(FOUR ? mx4::GROUP_BYTES : K), (cuuint64_t)rows, (cuuint64_t)(FOUR ? row_bytes / mx4::GROUP_BYTES : matrices),
+                          (cuuint64_t)matrices};
+    cuuint64_t strides[3] = {(cuuint64_t)row_bytes, (cuuint64_t)(FOUR ? mx4::GROUP_BYTES : row_bytes * rows), (cuuint64_t)(row_bytes * rows)};
+    cuuint32_t box[4] = {(cuuint32_t)(FOUR ? mx4::GROUP_BYTES : S::STEP), (cuuint32_t)(FOUR ? S::HALF : S::ROWS / box_matrices),
+                         (cuuint32_t)(FOUR ? S::SUB : box_matrices), (cuuint32_t)box_matrices};
+    cuuint32_t elem[4] = {1, 1, 1, 1};
     const CUresult r = enc(map, KIND == F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KIND == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
-                           3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           FOUR ? 4 : 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : FOUR ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return dd_fail("dd_moe_tokens: cannot describe %lld matrices of %lld x %d to TMA (driver error %d)", matrices, rows, K, (int)r);
     return 0;
 }
@@ -980,7 +988,7 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     c.cluster_shift = c.cluster == 8 ? 3 : c.cluster / 2;
     const size_t scratch = !c.l.router ? 0 : sizeof(Tile) * tiles * shares + sizeof(float) * (c.cluster * tiles * 16 * MAX_TOKENS +
                                                                                                 MAX_TOKENS * (2 * outputs + (c.l.groups > MAX_TOP ? c.l.groups : MAX_TOP)));
-    c.y_pitch = dd_ceil_div((long long)c.l.width, S::STEP) * S::STEP * S::ELEMENT + 16;
+    c.y_pitch = dd_ceil_div((long long)c.l.width, S::STEP) * S::STEP * S::ELEMENT + (KIND == MX4 ? 64 : 16);
     constexpr size_t MOST = 227 * 1024 - 32 * 1024;      // less the static part
     const size_t fixed = scratch + (size_t)c.T * c.y_pitch * (KIND == MX4 ? 2 : 1) + 1024, stage = UP_WARPS * S::STAGE_BYTES;
     if (fixed + 2 * stage > MOST)
