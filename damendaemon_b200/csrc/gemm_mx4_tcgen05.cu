@@ -10,16 +10,21 @@
 // that tcgen05.mma reads from tensor memory. A thread owns a row: it takes 128 elements (64 bytes, fetched by TMA) and their
 // four scales, and stores 64 pairs into its lane's columns; eight warps do nothing else until the epilogue. Two elements cost two
 // shifts, two masks and a multiplication, 2.4 operations an element with the store: 128 x 128 elements take four schedulers about
-// 400 clocks, the instructions that use them 4 T for a tile of T rows. So T = 128 where there are rows enough.
+// 400 clocks, the matrix instructions that use them 4 T for a tile of T rows. The decoding of a matrix for every tile of rows is what
+// these kernels cost beside a bfloat16 product; they are for rows that meet different matrices (grouped by expert) and for up to a few
+// hundred rows, where it hides behind the codes' way from memory.
 //
 // Rings: X (64 k a stage, TMA -> MMA), codes (128 k, TMA -> the eight warps), W in tensor memory (64 k, warps -> MMA). Without DUAL
-// the two sets of four warps take groups of 128 k in turn, with it one set the gate's and one the up rows. Every wait is bounded.
+// the two sets of four warps take groups of 128 k in turn, with it one set the gate's and one the up rows. Sets that take turns need rings
+// whose length they divide, so that a stage's phases are all waited for by one of them: a wait for the phase after one that has not
+// ended yet passes at once. Every wait is bounded.
 #include "common.cuh"
 #include "mx4.cuh"
 #include "tcgen05.cuh"
+#include <limits.h>
 
 namespace {
-constexpr int BM = 128, XK = 64, UMMA_K = 16, DEQUANT_WARPS = 8, THREADS = (DEQUANT_WARPS + 2) * 32;
+constexpr int BM = 128, XK = 64, UMMA_K = 16;
 constexpr int CODE_BYTES = BM * mx4::GROUP_BYTES;
 
 struct Mx4Params {
@@ -30,24 +35,36 @@ struct Mx4Params {
     const float* row_scale;      // [rows] or null
     void* out;                   // [rows, ldo]
     int* error_flag;
-    int rows, N, K, k_groups, rows_per_group, ldr, ldo, out_dtype, act, form;
+    int rows, N, K, k_groups, groups, rows_per_group, ldr, ldo, out_dtype, act, form;
     float limit, alpha;
 };
 
-template <int T, bool DUAL> struct Mx4Config {
+// The matrix of a tile of rows, or -1: skipped on purpose, or no such matrix (an error, and nothing is read or written).
+__device__ __forceinline__ int matrix_of(const Mx4Params& p, int tile) {
+    const int group = p.tile_group ? p.tile_group[tile] : 0;
+    if (group < p.groups) return group;
+    atomicOr(p.error_flag, 1);
+    return -1;
+}
+
+// SPLIT: the blocks of a cluster share K (tiles of 64 rows that are too few for the GPU otherwise).
+template <int T, bool DUAL, bool SPLIT = false> struct Mx4Config {
+    static constexpr int SETS = 2;                                   // of four warps that turn codes into rows
+    static constexpr int DEQUANT_WARPS = 4 * SETS, THREADS = (DEQUANT_WARPS + 2) * 32;
     static constexpr int X_BYTES = T * XK * 2;
     static constexpr int W_BYTES = (DUAL ? 2 : 1) * CODE_BYTES;
-    static constexpr int W_STAGES = DUAL ? 2 : 3;
-    static constexpr int X_FIT = (108 * 1024 - W_STAGES * W_BYTES) / X_BYTES;
-    static constexpr int X_STAGES = X_FIT < 8 ? X_FIT : 8;
-    static constexpr int A_STAGES = DUAL ? 2 : 4;                    // of 32 columns (64 k), twice that with DUAL
+    static constexpr int W_STAGES = DUAL ? 2 : 2 * SETS;             // (a set always meets the same stages: see the rings)
     static constexpr int ACC_COLS = (DUAL ? 2 : 1) * T;
-    static constexpr int A_COLS = 128;
-    static constexpr int WANTED = ACC_COLS + A_COLS;
-    static constexpr int TMEM_COLS = WANTED <= 256 ? 256 : 512;
+    static constexpr int A_STAGES = DUAL ? 2 : 2 * SETS;             // of 32 columns (64 k), twice that with DUAL
+    static constexpr int A_COLS = A_STAGES * (DUAL ? 64 : 32);
+    static constexpr int TMEM_COLS = ACC_COLS + A_COLS <= 256 ? 256 : 512;
     static constexpr int BLOCKS = TMEM_COLS == 256 ? 2 : 1;          // an SM
+    static constexpr int RED_BYTES = SPLIT ? BM * T * 4 : 0;         // the cluster's partial sums of this block's columns
+    static constexpr int X_FIT = ((BLOCKS == 2 ? 108 : 216) * 1024 - W_STAGES * W_BYTES - RED_BYTES) / X_BYTES;
+    static constexpr int X_STAGES = X_FIT < 8 ? X_FIT : 8;
     static constexpr int BARRIERS = 2 * (X_STAGES + W_STAGES + A_STAGES) + 1;
-    static constexpr int SMEM_BYTES = X_STAGES * X_BYTES + W_STAGES * W_BYTES + 1024 + BARRIERS * 8 + 16;
+    static constexpr int SMEM_BYTES = X_STAGES * X_BYTES + W_STAGES * W_BYTES + RED_BYTES + 1024 + BARRIERS * 8 + 16;
+    static_assert((DUAL || (W_STAGES % SETS == 0 && A_STAGES % (2 * SETS) == 0)) && ACC_COLS + A_COLS <= 512 && SMEM_BYTES <= 227 * 1024, "tensor or shared memory");
 };
 
 __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
@@ -55,20 +72,89 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// gelu_new(u) = u sigmoid(2 sqrt(2 / pi) (u + 0.044715 u^3)), for results that are rounded to bfloat16.
+__device__ __forceinline__ float gelu_new_fast(float u) {
+    return __fdividef(u, 1.0f + __expf(-1.5957691216057308f * (u + 0.044715f * u * u * u)));
+}
 // The factor of a block's pairs (mx4::pairs): 2^126 * 2^(s - 127), twice in a register; above 2^127 what is missing comes later.
 __device__ __forceinline__ uint32_t pair_factor(uint32_t s) {
     const uint32_t bits = s == 0 ? 0u : s == 255 ? 0x7fc0u : (min(s, 128u) + 126u) << 7;
     return bits | (bits << 16);
 }
 
-template <int T, bool DUAL>
-__global__ void __launch_bounds__(THREADS, Mx4Config<T, DUAL>::BLOCKS)
+template <int A> struct Act { static constexpr int value = A; };
+template <typename T> struct As { using Type = T; };
+
+// A thread's 128 elements of a row: word 4 t + b as words[t][b]. A row is 64 bytes under the 64-byte swizzle: 16-byte piece t lies at
+// t ^ (row / 2 % 4).
+__device__ __forceinline__ void read_codes(const uint8_t* tile, int row, uint32_t (*words)[4]) {
+    const uint4* from = reinterpret_cast<const uint4*>(tile + row * mx4::GROUP_BYTES);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const uint4 v = from[t ^ ((row >> 1) & 3)];
+        words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
+    }
+}
+// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales.
+__device__ __forceinline__ void half_of(const uint32_t (*words)[4], uint32_t four, int half, uint32_t* r) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const uint32_t scale = (four >> (16 * half + 8 * b)) & 255u, factor = pair_factor(scale);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            mx4::pairs(words[t][2 * half + b], r + b * 16 + t * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor);
+        }
+        if (scale > 128 && scale < 255) {
+            const uint32_t more = ((scale - 1) << 7) * 0x10001u;             // 2^(s - 128)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[b * 16 + j] = mul_pair(r[b * 16 + j], more);
+        }
+    }
+}
+// Results of feature n, rows r .. r + count - 1 (at most eight), from their sums; what the product's epilogue has is chosen outside of the
+// loop over them.
+template <bool DUAL>
+__device__ __forceinline__ void finish(const Mx4Params& p, int n, float bias, int r, int count, const float* g, const float* u) {
+    auto columns = [&](auto act, auto type) {
+        using Out = typename decltype(type)::Type;
+        Out* out = reinterpret_cast<Out*>(p.out) + (size_t)r * p.ldo + n;
+        const float* residual = p.residual ? p.residual + (size_t)r * p.ldr + n : nullptr;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j >= count) break;
+            float v = g[j];
+            if (DUAL) v = dd_gated_value<true>(v, u[j], p.form, p.limit, p.alpha);
+            else {
+                if (p.row_scale) v *= p.row_scale[r + j];
+                v += bias;
+                if (decltype(act)::value == DD_ACT_GELU_NEW) v = gelu_new_fast(v);
+                else if (decltype(act)::value != DD_ACT_NONE) v = dd_activation(v, p.act);
+            }
+            if (residual) v += residual[(size_t)j * p.ldr];
+            out[(size_t)j * p.ldo] = dd_from_f32<Out>(v);
+        }
+    };
+    // (the fast form is for results that are rounded to bfloat16; 'tanh' stands for every other activation)
+    if (p.out_dtype == DD_BF16) {
+        if (p.act == DD_ACT_NONE) columns(Act<DD_ACT_NONE>{}, As<__nv_bfloat16>{});
+        else if (p.act == DD_ACT_GELU_NEW) columns(Act<DD_ACT_GELU_NEW>{}, As<__nv_bfloat16>{});
+        else columns(Act<DD_ACT_TANH>{}, As<__nv_bfloat16>{});
+    } else if (p.act == DD_ACT_NONE) columns(Act<DD_ACT_NONE>{}, As<float>{});
+    else columns(Act<DD_ACT_TANH>{}, As<float>{});
+}
+
+template <int T, bool DUAL, bool SPLIT>
+__global__ void __launch_bounds__((Mx4Config<T, DUAL, SPLIT>::THREADS), (Mx4Config<T, DUAL, SPLIT>::BLOCKS))
 gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Mx4Params p) {
-    using C = Mx4Config<T, DUAL>;
+    using C = Mx4Config<T, DUAL, SPLIT>;
+    constexpr int DEQUANT_WARPS = C::DEQUANT_WARPS, SETS = C::SETS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* x_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* w_tiles = x_tiles + C::X_STAGES * C::X_BYTES;
-    uint64_t* x_full = reinterpret_cast<uint64_t*>(w_tiles + C::W_STAGES * C::W_BYTES);
+    float* partial = reinterpret_cast<float*>(w_tiles + C::W_STAGES * C::W_BYTES);      // [rank][T / splits columns][BM]
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(w_tiles + C::W_STAGES * C::W_BYTES + C::RED_BYTES);
     uint64_t* x_empty = x_full + C::X_STAGES;
     uint64_t* w_full = x_empty + C::X_STAGES;
     uint64_t* w_empty = w_full + C::W_STAGES;
@@ -97,11 +183,15 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot, tmem_a = tmem + C::ACC_COLS;
     dd_launch_dependents();
+    if (SPLIT) tc::cluster_arrive();             // (a block's shared memory may be written once it runs; waited for before the first write)
     dd_grid_wait();              // the tile's group and the rows are earlier kernels' results
 
-    const int n0 = blockIdx.x * BM, row0 = blockIdx.y * T;
-    const int group = p.tile_group ? p.tile_group[blockIdx.y] : 0;
-    const int kgroups = p.k_groups, kblocks = (p.K + XK - 1) / XK;
+    const int splits = SPLIT ? (int)tc::cluster_size() : 1, rank = SPLIT ? (int)tc::cluster_rank() : 0;
+    const int n0 = blockIdx.x / splits * BM, row0 = blockIdx.y * T;
+    const int group = matrix_of(p, blockIdx.y);
+    // this block's groups of 128 k, and its blocks of 64 (h counts from the first of them)
+    const int k_first = p.k_groups * rank / splits, kgroups = p.k_groups * (rank + 1) / splits - k_first;
+    const int kblocks = min(2 * kgroups, (p.K + XK - 1) / XK - 2 * k_first);
     if (group >= 0) {
         if (warp == DEQUANT_WARPS) {
             if (tc::elect_one()) {
@@ -113,13 +203,13 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     const int s = i % C::W_STAGES;
                     if (!tc::mbar_wait(&w_empty[s], ((i / C::W_STAGES) & 1) ^ 1, abort_flag)) break;
                     tc::mbar_expect_tx(&w_full[s], C::W_BYTES);
-                    tc::tma_load_2d(w_tiles + s * C::W_BYTES, &map_w, i * mx4::GROUP_BYTES, w_row, &w_full[s]);
-                    if (DUAL) tc::tma_load_2d(w_tiles + s * C::W_BYTES + CODE_BYTES, &map_w, i * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
+                    tc::tma_load_2d(w_tiles + s * C::W_BYTES, &map_w, (k_first + i) * mx4::GROUP_BYTES, w_row, &w_full[s]);
+                    if (DUAL) tc::tma_load_2d(w_tiles + s * C::W_BYTES + CODE_BYTES, &map_w, (k_first + i) * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
                     for (int h = 2 * i; h < min(2 * i + 2, kblocks); ++h) {
                         const int x = h % C::X_STAGES;
                         if (!tc::mbar_wait(&x_empty[x], ((h / C::X_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                         tc::mbar_expect_tx(&x_full[x], C::X_BYTES);
-                        tc::tma_load_2d(x_tiles + x * C::X_BYTES, &map_x, h * XK, row0, &x_full[x]);
+                        tc::tma_load_2d(x_tiles + x * C::X_BYTES, &map_x, (2 * k_first + h) * XK, row0, &x_full[x]);
                     }
                 }
             }
@@ -150,8 +240,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const int quarter = warp & 3, set = warp >> 2, row = quarter * 32 + lane;
             const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
             const size_t w_row = (size_t)group * p.rows_per_group + (DUAL && set ? p.N : 0) + min(n0 + row, p.N - 1);
-            const uint32_t* scales = p.scales + w_row * kgroups;
-            constexpr int STEP = DUAL ? 1 : 2;
+            const uint32_t* scales = p.scales + w_row * p.k_groups + k_first;
+            constexpr int STEP = DUAL ? 1 : SETS;
             const int first = DUAL ? 0 : set;
             uint32_t four = first < kgroups ? scales[first] : 0u;
             bool ok = true;
@@ -160,14 +250,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                 if (i + STEP < kgroups) four = scales[i + STEP];
                 const int s = i % C::W_STAGES;
                 if (!tc::mbar_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
-                // a row is 64 bytes under the 64-byte swizzle: 16-byte piece t lies at t ^ (row / 2 % 4)
-                const uint4* from = reinterpret_cast<const uint4*>(w_tiles + s * C::W_BYTES + (DUAL ? set * CODE_BYTES : 0) + row * mx4::GROUP_BYTES);
                 uint32_t words[4][4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const uint4 v = from[t ^ ((row >> 1) & 3)];
-                    words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
-                }
+                read_codes(w_tiles + s * C::W_BYTES + (DUAL ? set * CODE_BYTES : 0), row, words);
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&w_empty[s]);
 #pragma unroll
@@ -175,21 +259,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     const int h = 2 * i + half, a = h % C::A_STAGES;
                     if (h >= kblocks) break;
                     uint32_t r[32];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t scale = (by >> (16 * half + 8 * b)) & 255u, factor = pair_factor(scale);
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            mx4::pairs(words[t][2 * half + b], r + b * 16 + t * 4);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor);
-                        }
-                        if (scale > 128 && scale < 255) {
-                            const uint32_t more = ((scale - 1) << 7) * 0x10001u;             // 2^(s - 128)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) r[b * 16 + j] = mul_pair(r[b * 16 + j], more);
-                        }
-                    }
+                    half_of(words, by, half, r);
                     if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
                     tc::tmem_st_x32(tmem_a + lane_part + a * (DUAL ? 64 : 32) + (DUAL ? set * 32 : 0), r);
@@ -199,34 +269,49 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     if (lane == 0) tc::mbar_arrive(&a_full[a]);
                 }
             }
-            // epilogue: the two sets share the columns
             const int n = n0 + row;
-            if (tc::mbar_wait(acc_bar, 0, abort_flag)) {
-                tc::fence_after_sync();
-                const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+            const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+            const bool live = n < p.N;
+            // epilogue: the sets share the columns
+            const bool done = tc::mbar_wait(acc_bar, 0, abort_flag);
+            tc::fence_after_sync();
+            if (SPLIT) tc::cluster_wait();       // (every thread of the block waits here or below)
+            if (done)
 #pragma unroll 1
-                for (int c0 = set * (T / 2); c0 < (set + 1) * (T / 2); c0 += 8) {
+                for (int c0 = set * (T / SETS); c0 < (set + 1) * (T / SETS); c0 += 8) {
                     uint32_t g[8], u[8];
                     tc::tmem_ld_x8(tmem + lane_part + c0, g);
                     if (DUAL) tc::tmem_ld_x8(tmem + lane_part + T + c0, u);
                     tc::tmem_ld_wait();
-                    if (n < p.N) {
+                    if (SPLIT) {                 // to the block that finishes these columns
+                        const int width = T / splits, owner = c0 / width;
+                        const uint32_t to = tc::map_to_rank(&partial[(rank * width + c0 - owner * width) * BM + row], owner);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int r = row0 + c0 + j;
-                            if (r >= p.rows) break;
-                            float v = __uint_as_float(g[j]);
-                            if (DUAL) v = dd_gated_value<true>(v, __uint_as_float(u[j]), p.form, p.limit, p.alpha);
-                            else v = dd_activation((p.row_scale ? v * p.row_scale[r] : v) + bias, p.act);
-                            if (p.residual) v += p.residual[(size_t)r * p.ldr + n];
-                            const size_t at = (size_t)r * p.ldo + n;
-                            if (p.out_dtype == DD_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-                            else reinterpret_cast<float*>(p.out)[at] = v;
-                        }
-                    }
+                        for (int j = 0; j < 8; ++j) tc::st_cluster_f32(to + j * BM * 4, __uint_as_float(g[j]));
+                    } else if (live)
+                        finish<DUAL>(p, n, bias, row0 + c0, p.rows - row0 - c0, reinterpret_cast<const float*>(g), reinterpret_cast<const float*>(u));
+                }
+            if (SPLIT) {
+                tc::cluster_arrive();
+                tc::cluster_wait();
+                const int width = T / splits;
+#pragma unroll 1
+                for (int c = set; c < width; c += SETS) {
+                    float sum = 0.f;
+#pragma unroll 1
+                    for (int s = 0; s < splits; ++s) sum += partial[(s * width + c) * BM + row];      // in rank order
+                    const int r = row0 + rank * width + c;
+                    if (live && r < p.rows) finish<false>(p, n, bias, r, 1, &sum, nullptr);
                 }
             }
         }
+    }
+    // the warps without an epilogue take part in the cluster's barriers
+    if (SPLIT && warp >= DEQUANT_WARPS) {
+        __syncwarp();
+        tc::cluster_wait();
+        tc::cluster_arrive();
+        tc::cluster_wait();
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -234,6 +319,190 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (warp == DEQUANT_WARPS + 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+// The same without the gated unit where there are more tiles than SMs: a block an SM that takes tile after tile, with two accumulators, so
+// that the epilogue of a tile (eight warps of its own) runs under the products of the next. 4,096 rows of sixteen experts of 2,048 x 2,048 in
+// tiles of 128 rows, float32 results: TBD us, a block a tile 65. What holds it: X, which every block reads for 128 features (L2 gives
+// 12 TB/s), then the instructions of decoding and epilogue.
+template <int T> struct LoopConfig {
+    static constexpr int SETS = 4, DEQUANT_WARPS = 16, EPILOGUE_WARPS = 8, THREADS = (DEQUANT_WARPS + EPILOGUE_WARPS + 2) * 32;
+    static constexpr int X_BYTES = T * XK * 2, W_STAGES = 2 * SETS;
+    static constexpr int A_STAGES = (512 - 2 * T) / 32 < 8 ? (512 - 2 * T) / 32 : 8;
+    static constexpr int X_FIT = (210 * 1024 - W_STAGES * CODE_BYTES) / X_BYTES, X_STAGES = X_FIT < 8 ? X_FIT : 8;
+    static constexpr int BARRIERS = 2 * (X_STAGES + W_STAGES + A_STAGES + 2);
+    static constexpr int SMEM_BYTES = X_STAGES * X_BYTES + W_STAGES * CODE_BYTES + 1024 + BARRIERS * 8 + 16;
+    static_assert(W_STAGES % SETS == 0 && A_STAGES % (2 * SETS) == 0 && 2 * T + A_STAGES * 32 <= 512 && SMEM_BYTES <= 227 * 1024, "tensor or shared memory");
+};
+
+template <int T>
+__global__ void __launch_bounds__(LoopConfig<T>::THREADS, 1)
+gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Mx4Params p) {
+    using C = LoopConfig<T>;
+    constexpr int TMA_WARP = C::DEQUANT_WARPS, MMA_WARP = TMA_WARP + 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* x_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* w_tiles = x_tiles + C::X_STAGES * C::X_BYTES;
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(w_tiles + C::W_STAGES * CODE_BYTES);
+    uint64_t* x_empty = x_full + C::X_STAGES;
+    uint64_t* w_full = x_empty + C::X_STAGES;
+    uint64_t* w_empty = w_full + C::W_STAGES;
+    uint64_t* a_full = w_empty + C::W_STAGES;
+    uint64_t* a_empty = a_full + C::A_STAGES;
+    uint64_t* acc_full = a_empty + C::A_STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::X_STAGES; ++s) { tc::mbar_init(&x_full[s], 1); tc::mbar_init(&x_empty[s], 1); }
+        for (int s = 0; s < C::W_STAGES; ++s) { tc::mbar_init(&w_full[s], 1); tc::mbar_init(&w_empty[s], 4); }
+        for (int s = 0; s < C::A_STAGES; ++s) { tc::mbar_init(&a_full[s], 4); tc::mbar_init(&a_empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { tc::mbar_init(&acc_full[s], 1); tc::mbar_init(&acc_empty[s], C::EPILOGUE_WARPS); }
+        *abort_flag = 0;
+        tc::fence_barrier_init();
+        tc::fence_proxy_async();
+        tc::prefetch_tensormap(&map_w);
+        tc::prefetch_tensormap(&map_x);
+    }
+    if (warp == MMA_WARP) {
+        tc::tmem_alloc(tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot, tmem_a = tmem + 2 * T;
+    dd_launch_dependents();
+    dd_grid_wait();              // the tiles' groups and the rows are earlier kernels' results
+
+    const int n_tiles = (p.N + BM - 1) / BM, total = n_tiles * ((p.rows + T - 1) / T);
+    // (both halves of the last group, also where K ends in the first: a set then always meets the same stages; zeros by zeros)
+    const int kgroups = p.k_groups, kblocks = 2 * kgroups;
+    // Every role walks the same tiles; the number of a stage counts on over them. w: groups of 128 k, h: blocks of 64, n: tiles.
+    auto group_of = [&](int tile) { return matrix_of(p, tile / n_tiles); };
+    if (warp == TMA_WARP) {
+        if (tc::elect_one()) {
+            int w = 0, h = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                const int group = group_of(tile), n0 = tile % n_tiles * BM, row0 = tile / n_tiles * T;
+                if (group < 0) continue;
+                for (int i = 0; i < kgroups && ok; ++i, ++w) {
+                    const int s = w % C::W_STAGES;
+                    if (!tc::mbar_wait(&w_empty[s], ((w / C::W_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    tc::mbar_expect_tx(&w_full[s], CODE_BYTES);
+                    tc::tma_load_2d(w_tiles + s * CODE_BYTES, &map_w, i * mx4::GROUP_BYTES, group * p.rows_per_group + n0, &w_full[s]);
+                    for (int half = 2 * i; half < 2 * i + 2; ++half, ++h) {
+                        const int x = h % C::X_STAGES;
+                        if (!tc::mbar_wait(&x_empty[x], ((h / C::X_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        tc::mbar_expect_tx(&x_full[x], C::X_BYTES);
+                        tc::tma_load_2d(x_tiles + x * C::X_BYTES, &map_x, half * XK, row0, &x_full[x]);
+                    }
+                }
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        if (tc::elect_one()) {
+            constexpr uint32_t idesc = tc::idesc_bf16_f32(BM, T);
+            int h = 0, n = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                if (group_of(tile) < 0) continue;
+                const uint32_t acc = tmem + (n & 1) * T;
+                if (!tc::mbar_wait(&acc_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
+                tc::fence_after_sync();
+                for (int i = 0; i < kblocks; ++i, ++h) {
+                    const int x = h % C::X_STAGES, a = h % C::A_STAGES;
+                    if (!tc::mbar_wait(&x_full[x], (h / C::X_STAGES) & 1, abort_flag) ||
+                        !tc::mbar_wait(&a_full[a], (h / C::A_STAGES) & 1, abort_flag)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    const uint32_t x_addr = tc::smem_u32(x_tiles + x * C::X_BYTES);
+#pragma unroll
+                    for (int k = 0; k < XK / UMMA_K; ++k)
+                        tc::mma_bf16_a_tmem(acc, tmem_a + a * 32 + k * (UMMA_K / 2), tc::smem_desc_sw128(x_addr + k * UMMA_K * 2), idesc,
+                                            (i > 0 || k > 0) ? 1u : 0u);
+                    tc::mma_commit(&x_empty[x]);
+                    tc::mma_commit(&a_empty[a]);
+                }
+                if (ok) tc::mma_commit(&acc_full[n & 1]);
+                ++n;
+            }
+        }
+    } else if (warp < C::DEQUANT_WARPS) {
+        const int quarter = warp & 3, set = warp >> 2, row = quarter * 32 + lane;
+        const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
+        int w0 = 0, h0 = 0;                      // of the tile's first group and block
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+            const int group = group_of(tile), n0 = tile % n_tiles * BM;
+            if (group < 0) continue;
+            const uint32_t* scales = p.scales + ((size_t)group * p.rows_per_group + min(n0 + row, p.N - 1)) * kgroups;
+            const int first = (set - w0 % C::SETS + C::SETS) % C::SETS;
+            uint32_t four = first < kgroups ? scales[first] : 0u;
+            for (int i = first; i < kgroups && ok; i += C::SETS) {
+                const uint32_t by = four;
+                if (i + C::SETS < kgroups) four = scales[i + C::SETS];
+                const int w = w0 + i, s = w % C::W_STAGES;
+                if (!tc::mbar_wait(&w_full[s], (w / C::W_STAGES) & 1, abort_flag)) { ok = false; break; }
+                uint32_t words[4][4];
+                read_codes(w_tiles + s * CODE_BYTES, row, words);
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&w_empty[s]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int h = h0 + 2 * i + half, a = h % C::A_STAGES;
+                    uint32_t r[32];
+                    half_of(words, by, half, r);
+                    if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    tc::tmem_st_x32(tmem_a + lane_part + a * 32, r);
+                    tc::tmem_st_wait();
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&a_full[a]);
+                }
+            }
+            w0 += kgroups;
+            h0 += kblocks;
+        }
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
+        int number = 0;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            if (group_of(tile) < 0) continue;
+            const int n = tile % n_tiles * BM + row, row0 = tile / n_tiles * T;
+            const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+            if (!tc::mbar_wait(&acc_full[number & 1], (number >> 1) & 1, abort_flag)) break;
+            tc::fence_after_sync();
+            // two warps a quarter of the lanes, half of the columns each
+            const int half = (warp - MMA_WARP - 1) >> 2, count = min(T, p.rows - row0);
+#pragma unroll 1
+            for (int c0 = half * (T / 2); c0 < min(count, (half + 1) * (T / 2)); c0 += 16) {
+                uint32_t g[16];
+                tc::tmem_ld_x16(tmem + (number & 1) * T + lane_part + c0, g);
+                tc::tmem_ld_wait();
+                if (n < p.N)
+#pragma unroll
+                    for (int j = 0; j < 16; j += 8)
+                        if (c0 + j < count) finish<false>(p, n, bias, row0 + c0 + j, count - c0 - j, reinterpret_cast<const float*>(g + j), nullptr);
+                __syncwarp();
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&acc_empty[number & 1]);
+            ++number;
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 8);
+    if (warp == MMA_WARP) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
     }
 }
 
@@ -262,23 +531,47 @@ int mx4_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long l
     return 0;
 }
 
-template <int T, bool DUAL>
-int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, cudaStream_t s) {
-    using C = Mx4Config<T, DUAL>;
-    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+template <int T, bool DUAL, bool SPLIT = false>
+int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, cudaStream_t s, int splits = 1) {
+    using C = Mx4Config<T, DUAL, SPLIT>;
+    cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, DUAL, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
-    dd_launch(gemm_mx4_kernel<T, DUAL>, dim3(dd_ceil_div(p.N, BM), dd_ceil_div(p.rows, T)), dim3(THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(dd_ceil_div(p.N, BM) * splits, dd_ceil_div(p.rows, T));
+    config.blockDim = dim3(C::THREADS);
+    config.dynamicSmemBytes = C::SMEM_BYTES;
+    config.stream = s;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = dd_pdl_enabled ? 1 : 0;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = splits;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    config.attrs = attrs;
+    config.numAttrs = SPLIT ? 2 : 1;
+    e = cudaLaunchKernelEx(&config, gemm_mx4_kernel<T, DUAL, SPLIT>, mw, mx, p);
+    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4 (clusters of %d): %s", splits, cudaGetErrorString(e));
+    return dd_check_launch("dd_gemm_mx4");
+}
+template <int T>
+int launch_loop(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, int sms, cudaStream_t s) {
+    using C = LoopConfig<T>;
+    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_loop_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
+    const int tiles = dd_ceil_div(p.N, BM) * dd_ceil_div(p.rows, T);
+    dd_launch(gemm_mx4_loop_kernel<T>, dim3(tiles < sms ? tiles : sms), dim3(C::THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);
     return dd_check_launch("dd_gemm_mx4");
 }
 }  // namespace
 
-// X [rows, K] bf16 (row stride ldx) in tiles of `tile` rows (16, 32, 64 or 128); codes, scales: `groups` 4-bit matrices of
-// rows_per_group rows of K; tile_group: device array [rows / tile] (a negative group's tile is skipped), or null: one matrix for
+// X [rows, K] bf16 (row stride ldx) in tiles of `tile` rows (16, 32, 64, 128); codes, scales: `groups` 4-bit matrices of rows_per_group
+// rows of K; tile_group: device array [rows / tile] (a negative group's tile is skipped, so is one out of range, with error bit 1), or null: one matrix for
 // all rows, of which the last tile may hold fewer. dual == 0: rows_per_group == N, act(row_scale * sum + bias) + residual; dual != 0:
 // rows_per_group == 2 N, the gated unit. out: [rows, N] bf16 or f32, row stride ldo.
 DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* scales, int groups, int rows_per_group, const int* tile_group,
                        const float* bias, const float* residual, int ldr, const float* row_scale, void* out, int ldo, int rows, int N, int K,
-                       int tile, int dual, float limit, float alpha, int form, int act, int out_dtype, int* error_flag, void* stream) {
+                       int tile, int dual, float limit, float alpha, int form, int act, int out_dtype, int sms, int* error_flag, void* stream) {
     if (rows <= 0 || N <= 0) return 0;
     if (K <= 0 || K % 8 || ldx % 8) return dd_fail("dd_gemm_mx4: K=%d and the row stride %d must be multiples of 8 (TMA needs 16-byte rows)", K, ldx);
     if (((uintptr_t)X & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3)) return dd_fail("dd_gemm_mx4: operands must be 16-byte aligned");
@@ -286,9 +579,10 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
     if (tile <= 0 || (tile_group && rows % tile) || dd_ceil_div(rows, tile) > 65535) return dd_fail("dd_gemm_mx4: %d rows in tiles of %d", rows, tile);
     if (groups <= 0 || (groups > 1 && !tile_group) || rows_per_group != (dual ? 2 * N : N))
         return dd_fail("dd_gemm_mx4: %d groups of %d rows do not fit N=%d", groups, rows_per_group, N);
+    if ((long long)groups * rows_per_group > INT_MAX) return dd_fail("dd_gemm_mx4: %d groups of %d rows pass 32 bits", groups, rows_per_group);
     Mx4Params p;
     p.scales = (const uint32_t*)scales; p.tile_group = tile_group; p.bias = bias; p.residual = residual; p.row_scale = row_scale; p.out = out;
-    p.error_flag = error_flag; p.rows = rows; p.N = N; p.K = K; p.k_groups = dd_ceil_div(K, mx4::GROUP); p.rows_per_group = rows_per_group;
+    p.error_flag = error_flag; p.rows = rows; p.N = N; p.K = K; p.k_groups = dd_ceil_div(K, mx4::GROUP); p.groups = groups; p.rows_per_group = rows_per_group;
     p.ldr = ldr; p.ldo = ldo; p.out_dtype = out_dtype; p.act = act; p.form = form; p.limit = limit; p.alpha = alpha;
     const long long row_bytes = (long long)p.k_groups * mx4::GROUP_BYTES;
     CUtensorMap mw, mx;
@@ -297,6 +591,13 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
     if (int e = mx4_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, X, rows, K, (long long)ldx * 2, XK, tile, CU_TENSOR_MAP_SWIZZLE_128B, "the rows"))
         return e;
     cudaStream_t s = (cudaStream_t)stream;
+    // Tiles of 64 rows that would leave most of the GPU idle share K among two, four or eight blocks, as long as each keeps two groups
+    // and all fit at once (two an SM).
+    int splits = 1;
+    const int tiles = dd_ceil_div(N, BM) * dd_ceil_div(rows, tile);
+    while (tile == 64 && !dual && !tile_group && splits < 8 && tiles * splits * 2 <= 296 && p.k_groups >= splits * 4) splits *= 2;
+    if (splits > 1) return launch_mx4<64, false, true>(mw, mx, p, s, splits);
+    if (tile == 128 && !dual && tiles > sms) return launch_loop<128>(mw, mx, p, sms, s);      // more tiles than SMs
 #define DD_MX4(T) \
     case T: return dual ? launch_mx4<T, true>(mw, mx, p, s) : launch_mx4<T, false>(mw, mx, p, s);
     switch (tile) {

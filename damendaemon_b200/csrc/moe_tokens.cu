@@ -72,8 +72,8 @@ struct Tile { float sum[16][few::COLUMNS + 1]; };
 template <int N> struct Count { static constexpr int value = N; };
 
 // What a warp multiplies at a time, a tile: 16 rows of a matrix on mma.sync, 4 with multiply-adds. A stage of its ring is one TMA box
-// of a tile (two boxes of half the rows, or half the columns, took 4-bit matrices at 2 TB/s: a copy costs about 50 clocks
-// whatever its size).
+// of a tile where its rows lie together (a copy has a cost of its own: eight tokens, eight each of 64 experts of 2 x 1,024 x 2,048, 4 bits: up_kernel 37 us
+// and 44 with two boxes a stage).
 template <int KIND> struct Stream {
     static constexpr int ROWS = KIND == F32 ? few::F32_ROWS : 16, HALF = ROWS / 2;
     static constexpr int STEP = KIND == BF16 ? 64 : KIND == F32 ? 128 : 256;         // k
@@ -144,7 +144,7 @@ __device__ __forceinline__ void take_column(uint4* b, const __nv_bfloat16* x, in
     for (int i = 0; i < PIECES<KIND>; ++i) b[i] = from[KIND == MX4 ? 4 * i + t : 2 * t + i];
 }
 // The scales of sixteen 4-bit groups of rows g and g + 8: lane (g, t) holds those of groups 4 t .. 4 t + 3, and asks for them a
-// stretch of sixteen ahead (a lane's four bytes a step, requested one step ahead, came from L2 or beyond at every step: 1 us).
+// stretch of sixteen ahead.
 struct Scales {
     static constexpr int STRETCH = 16;
     uint32_t a[4], b[4];
@@ -191,15 +191,24 @@ __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0,
             }
         }
     } else {
+        // (the tensor cores cut off where they add: a sum of 64 products starts from nothing and is added rounded)
+        uint4 a[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t at = slot + g * 128 + ((2 * t + i) ^ g) * 16;
-            const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
+            a[i][0] = few::lds16(at);
+            a[i][1] = few::lds16(at + 1024);
+        }
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                few::mma(d[p], a0.x, a1.x, a0.y, a1.y, b[p][i].x, b[p][i].y);
-                few::mma(d[p], a0.z, a1.z, a0.w, a1.w, b[p][i].z, b[p][i].w);
+        for (int p = 0; p < P; ++p) {
+            float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                few::mma(e, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b[p][i].x, b[p][i].y);
+                few::mma(e, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b[p][i].z, b[p][i].w);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[p][j] += e[j];
         }
     }
 }
@@ -974,26 +983,46 @@ int launch_down(const Call& c, const Maps& m, int tiles, cudaStream_t s) {
     return dd_check_launch("dd_moe_tokens");
 }
 
+// How up_kernel shares its routing and its shared memory out.
+struct UpPlan { int tiles, shares, cluster, y_pitch; size_t fixed, stage; };
+constexpr size_t MOST_SHARED = 227 * 1024 - 32 * 1024;       // less the static part
+template <int KIND>
+UpPlan plan_up(const DdExpertLayer& l, int T) {
+    using S = Stream<KIND>;
+    UpPlan u;
+    const int outputs = l.experts + l.identity, rows = outputs + l.shared_gate;
+    // a router of up to 64 KB is read by every block for itself, a larger one shared by a cluster's blocks
+    // (128 outputs and more leave no room for what eight blocks send)
+    const size_t router_bytes = l.router ? (size_t)rows * l.width * S::ELEMENT : 0;
+    u.tiles = (rows + 15) / 16;
+    u.shares = u.tiles >= 9 ? 1 : u.tiles >= 5 ? 2 : u.tiles >= 3 ? 4 : u.tiles == 2 ? 8 : 16;
+    u.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) || u.tiles > 8 ? 4 : 8;
+    const size_t scratch = !l.router ? 0 : sizeof(Tile) * u.tiles * u.shares + sizeof(float) * (u.cluster * u.tiles * 16 * MAX_TOKENS +
+                                                                              MAX_TOKENS * (2 * outputs + (l.groups > MAX_TOP ? l.groups : MAX_TOP)));
+    u.y_pitch = dd_ceil_div((long long)l.width, S::STEP) * S::STEP * S::ELEMENT + (KIND == MX4 ? 64 : 16);
+    u.fixed = scratch + (size_t)T * u.y_pitch * (KIND == MX4 ? 2 : 1) + 1024;
+    u.stage = UP_WARPS * S::STAGE_BYTES;
+    return u;
+}
+template <int KIND>
+int most_tokens(const DdExpertLayer& l) {        // with two stages a ring
+    for (int T = MAX_TOKENS; T > 0; --T) {
+        const UpPlan u = plan_up<KIND>(l, T);
+        if (u.fixed + 2 * u.stage <= MOST_SHARED) return T;
+    }
+    return 0;
+}
+
 template <int KIND>
 int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     using S = Stream<KIND>;
-    const int outputs = c.l.experts + c.l.identity, rows = outputs + c.l.shared_gate;
-    // a router of up to 64 KB is read by every block for itself, a larger one shared by a cluster's blocks
-    // (128 outputs and more leave no room for what eight blocks send)
-    const size_t router_bytes = c.l.router ? (size_t)rows * c.l.width * S::ELEMENT : 0;
-    const int tiles = (rows + 15) / 16, shares = tiles >= 9 ? 1 : tiles >= 5 ? 2 : tiles >= 3 ? 4 : tiles == 2 ? 8 : 16;
-    c.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) || tiles > 8 ? 4 : 8;
-    c.router_tiles = tiles;
-    c.share_shift = shares == 16 ? 4 : shares / 2 - (shares == 8);
-    c.cluster_shift = c.cluster == 8 ? 3 : c.cluster / 2;
-    const size_t scratch = !c.l.router ? 0 : sizeof(Tile) * tiles * shares + sizeof(float) * (c.cluster * tiles * 16 * MAX_TOKENS +
-                                                                                                MAX_TOKENS * (2 * outputs + (c.l.groups > MAX_TOP ? c.l.groups : MAX_TOP)));
-    c.y_pitch = dd_ceil_div((long long)c.l.width, S::STEP) * S::STEP * S::ELEMENT + (KIND == MX4 ? 64 : 16);
-    constexpr size_t MOST = 227 * 1024 - 32 * 1024;      // less the static part
-    const size_t fixed = scratch + (size_t)c.T * c.y_pitch * (KIND == MX4 ? 2 : 1) + 1024, stage = UP_WARPS * S::STAGE_BYTES;
-    if (fixed + 2 * stage > MOST)
+    const UpPlan u = plan_up<KIND>(c.l, c.T);
+    if (u.fixed + 2 * u.stage > MOST_SHARED)
         return dd_fail("dd_moe_tokens: %d rows of %d elements are more than a block's shared memory holds beside its rings", c.T, c.l.width);
-    c.stages = (int)((MOST - fixed) / stage);
+    c.cluster = u.cluster; c.y_pitch = u.y_pitch; c.router_tiles = u.tiles;
+    c.share_shift = u.shares == 16 ? 4 : u.shares / 2 - (u.shares == 8);
+    c.cluster_shift = u.cluster == 8 ? 3 : u.cluster / 2;
+    c.stages = (int)((MOST_SHARED - u.fixed) / u.stage);
     if (c.stages > S::MOST_STAGES) c.stages = S::MOST_STAGES;
     // what the GPU holds at once, a block an SM (a second wave of blocks would double the time): a B200's SMs take 33 clusters
     // of four, 15 of eight
@@ -1003,7 +1032,7 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     if (at_most > (1 << 21) || (long long)c.l.experts * c.l.inner * 2 > INT_MAX || (long long)c.l.experts * c.l.width > INT_MAX)
         return dd_fail("dd_moe_tokens: %d experts of %d x %d are too large", c.l.experts, c.l.inner, c.l.width);
     const int blocks = at_most < most ? (int)((at_most + c.cluster - 1) / c.cluster * c.cluster) : most;
-    if (int e = launch_up<KIND>(c, m, blocks, fixed + c.stages * stage, s)) return e;
+    if (int e = launch_up<KIND>(c, m, blocks, u.fixed + c.stages * u.stage, s)) return e;
     // a block a tile; as many warps on it as let all blocks run at once
     const int down_tiles = dd_ceil_div(c.l.width, S::ROWS);
     if (down_tiles <= sms) return launch_down<KIND, 16>(c, m, down_tiles, s);
@@ -1021,6 +1050,10 @@ int units_of(const DdExpertLayer& l, int T) { return T * l.top < l.experts ? T *
 // Bytes of scratch that a call of T tokens needs (16-byte aligned).
 DD_API long long dd_moe_tokens_scratch(const DdExpertLayer* l, int T) {
     return (long long)(sizeof(Plan) + hidden_bytes(*l, T, units_of(*l, T)));
+}
+// The most tokens that a call with this layer can take (its rows have to fit into shared memory beside the rings).
+DD_API int dd_moe_tokens_most(const DdExpertLayer* l) {
+    return l->kind == F32 ? most_tokens<F32>(*l) : l->kind == BF16 ? most_tokens<BF16>(*l) : most_tokens<MX4>(*l);
 }
 // The layer's matrices as TMA takes them: 512 bytes, 64-byte aligned, which every call copies. They hold while the matrices lie where they are.
 DD_API int dd_moe_tokens_maps(const DdExpertLayer* l, void* maps) {

@@ -32,20 +32,30 @@ __device__ __forceinline__ void load_row8(const T* row, int k, int n, bool wide,
     for (int i = 0; i < 8; ++i) x[i] = k + i < n ? dd_to_f32(row[k + i]) : 0.f;
 }
 
+// (UNROLL groups of a row's neighbours, or of the next row, in flight a thread: with one 6,400 x 1,600 took twice as long)
+constexpr int UNROLL = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 quantize_kernel(const T* x, long long ldx, int width, int groups, long long n_groups, uint32_t* codes, uint32_t* scales, int wide) {
     dd_grid_wait();
     const int lane = threadIdx.x & 15, b = lane >> 2, t = lane & 3;
-    for (long long at = ((long long)blockIdx.x * THREADS + threadIdx.x) >> 4; at < n_groups; at += (long long)gridDim.x * (THREADS / 16)) {
-        const long long row = at / groups;
-        const int k = (int)(at - row * groups) * mx4::GROUP + b * mx4::BLOCK + t * 8;
-        float v[8];
-        load_row8(x + row * ldx, k, width, wide, v);
+    const unsigned mask = 0xffffu << (threadIdx.x & 16);
+    const long long first = (((long long)blockIdx.x * THREADS + threadIdx.x) >> 4) * UNROLL;
+    long long row = first / groups;
+    int group = (int)(first - row * groups);
+    float v[UNROLL][8];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        if (first + u < n_groups) load_row8(x + row * ldx, group * mx4::GROUP + b * mx4::BLOCK + t * 8, width, wide, v[u]);
+        if (++group == groups) { group = 0; ++row; }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        if (first + u >= n_groups) break;
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-        const unsigned mask = 0xffffu << (threadIdx.x & 16);
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
         top = max(top, __shfl_xor_sync(mask, top, 1));
         top = max(top, __shfl_xor_sync(mask, top, 2));
         const uint32_t exponent = top >> 23;
@@ -57,39 +67,49 @@ quantize_kernel(const T* x, long long ldx, int width, int groups, long long n_gr
             const int e = i < 2 ? 4 * i : 4 * (i - 2) + 1;
             uint16_t byte;
             asm("{\n\t.reg .b8 q;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %1, %2;\n\tcvt.u16.u8 %0, q;\n\t}"
-                : "=h"(byte) : "f"(v[e + 2] * by), "f"(v[e] * by));
+                : "=h"(byte) : "f"(v[u][e + 2] * by), "f"(v[u][e] * by));
             word |= (uint32_t)byte << (8 * i);
         }
-        codes[at * 16 + 4 * t + b] = s == 255 ? 0u : word;
+        codes[(first + u) * 16 + 4 * t + b] = s == 255 ? 0u : word;
         uint32_t four = s << (8 * b);
         four |= __shfl_xor_sync(mask, four, 4);
         four |= __shfl_xor_sync(mask, four, 8);
-        if (lane == 0) scales[at] = four;
+        if (lane == 0) scales[first + u] = four;
     }
 }
 
 // ---------------------------------------------------------------- the values back
+// (Nor may the kernels after this one start before it has ended: it makes the matrix that a product may fetch before its wait.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 values_kernel(const uint32_t* codes, const uint32_t* scales, int width, int groups, long long n_groups, T* out, int wide) {
-    dd_launch_dependents();
     dd_grid_wait();
     const int lane = threadIdx.x & 15, b = lane >> 2, t = lane & 3;
-    for (long long at = ((long long)blockIdx.x * THREADS + threadIdx.x) >> 4; at < n_groups; at += (long long)gridDim.x * (THREADS / 16)) {
-        const long long row = at / groups;
-        const int k = (int)(at - row * groups) * mx4::GROUP + b * mx4::BLOCK + t * 8;
-        if (k >= width) continue;
-        const uint32_t s = (scales[at] >> (8 * b)) & 255u;
+    const long long first = (((long long)blockIdx.x * THREADS + threadIdx.x) >> 4) * UNROLL;
+    uint32_t word[UNROLL], four[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        word[u] = first + u < n_groups ? codes[(first + u) * 16 + 4 * t + b] : 0u;
+        four[u] = first + u < n_groups ? scales[first + u] : 0u;
+    }
+    long long row = first / groups;
+    int group = (int)(first - row * groups);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int k = group * mx4::GROUP + b * mx4::BLOCK + t * 8;
+        T* to = out + row * width + k;
+        if (++group == groups) { group = 0; ++row; }
+        if (first + u >= n_groups || k >= width) continue;
+        const uint32_t s = (four[u] >> (8 * b)) & 255u;
         const float by = __uint_as_float(s == 255 ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
         uint32_t pair[4];
-        mx4::pairs(codes[at * 16 + 4 * t + b], pair);
+        mx4::pairs(word[u], pair);
         __align__(16) T v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {           // the pair's element is times 2^-126
             const float e = __uint_as_float(i & 1 ? pair[i >> 1] & 0xffff0000u : pair[i >> 1] << 16) * 8.507059173023462e37f;
             v[i] = dd_from_f32<T>(e * by);
         }
-        T* to = out + row * width + k;
         if (wide) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(v) / 16; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(v)[i];
@@ -220,8 +240,9 @@ DD_API int dd_mx4_quantize(const void* x, long long ldx, long long rows, int wid
     if (rows <= 0 || width <= 0) return 0;
     const int groups = dd_ceil_div(width, mx4::GROUP);
     const long long n = rows * groups;
-    const long long blocks = (n + THREADS / 16 - 1) / (THREADS / 16);
-    const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+    const long long blocks = (n + THREADS / 16 * UNROLL - 1) / (THREADS / 16 * UNROLL);
+    if (blocks > 0x7fffffffll) return dd_fail("dd_mx4: %lld rows of %d are too many", rows, width);
+    const dim3 grid((unsigned)blocks);
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DD_F32)
         dd_launch(quantize_kernel<float>, grid, dim3(THREADS), 0, s, (const float*)x, ldx, width, groups, n, (uint32_t*)codes,
@@ -239,8 +260,9 @@ DD_API int dd_mx4_values(const void* codes, const void* scales, long long rows, 
     if (rows <= 0 || width <= 0) return 0;
     const int groups = dd_ceil_div(width, mx4::GROUP);
     const long long n = rows * groups;
-    const long long blocks = (n + THREADS / 16 - 1) / (THREADS / 16);
-    const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+    const long long blocks = (n + THREADS / 16 * UNROLL - 1) / (THREADS / 16 * UNROLL);
+    if (blocks > 0x7fffffffll) return dd_fail("dd_mx4: %lld rows of %d are too many", rows, width);
+    const dim3 grid((unsigned)blocks);
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DD_F32)
         dd_launch(values_kernel<float>, grid, dim3(THREADS), 0, s, (const uint32_t*)codes, (const uint32_t*)scales, width, groups, n,

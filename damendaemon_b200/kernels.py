@@ -105,6 +105,7 @@ _SIGNATURES = {
                          _c_int, _c_int, _c_void],
         "dd_round_rows": [_c_void, _c_void, ctypes.c_longlong, _c_void],
         "dd_moe_tokens_maps": [_c_void, _c_void],
+        "dd_moe_tokens_most": [_c_void],
         "dd_moe_tokens": [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
         "dd_mx4_quantize": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_int, _c_void],
         "dd_mx4_values": [_c_void, _c_void, ctypes.c_longlong, _c_int, _c_void, _c_int, _c_void],
@@ -117,7 +118,7 @@ _SIGNATURES = {
         "dd_gemm_grouped_tcgen05": [_c_void, _c_int, _c_void, _c_int, _c_int, _c_int, _c_void, _c_void, _c_int] + [_c_int] * 5
                                    + [_c_float, _c_float, _c_int, _c_void, _c_void, _c_int, _c_int, _c_void],
         "dd_gemm_mx4": [_c_void, _c_int, _c_void, _c_void, _c_int, _c_int] + [_c_void] * 3 + [_c_int, _c_void, _c_void] + [_c_int] * 6
-                       + [_c_float, _c_float, _c_int, _c_int, _c_int, _c_void, _c_void],
+                       + [_c_float, _c_float, _c_int, _c_int, _c_int, _c_int, _c_void, _c_void],
         "dd_wait_probe": [ctypes.c_ulonglong, _c_void, _c_void, _c_void],
         "dd_attention_decode_supported": [_c_int] * 4,
         "dd_attention_prefill_supported": [_c_int] * 4,
@@ -1606,23 +1607,25 @@ class ExpertLayer:
         self._map_store = ctypes.create_string_buffer(512 + 64)      # the matrices as TMA takes them, at a 64-byte boundary
         self._maps = (ctypes.addressof(self._map_store) + 63) // 64 * 64
         _call(library("core"), "dd_moe_tokens_maps", self._at, self._maps, n_kernels=0)
-        self._scratch = [0] + [int(library("core").dd_moe_tokens_scratch(self._at, t)) for t in range(1, MOE_TOKENS + 1)]
+        # rows so wide that they do not fit into shared memory beside the rings go to the kernels of larger steps
+        self.most_tokens = int(library("core").dd_moe_tokens_most(self._at))
+        self._scratch = [0] + [int(library("core").dd_moe_tokens_scratch(self._at, t)) for t in range(1, self.most_tokens + 1)]
 
 
 def expert_layer_fits(top, router_rows):
-    """Whether moe_tokens chooses among that many router rows (experts, identity outputs, a shared unit's gate)."""
+    """Whether an ExpertLayer can have that many choices a token and router rows (experts, identity outputs, a shared unit's gate)."""
     return top <= MOE_TOP and router_rows <= MOE_OUTPUTS
 
 
 def moe_tokens(layer, y, residual=None, ids=None, out=None):
-    """A whole expert layer for one to MOE_TOKENS tokens in two kernels: routing, the chosen units, the shared unit, the weighted
-    sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the layer's dtype; ids int32 [T] for a layer by
-    table; out float32 (residual itself may be given). Sums are float32; a hidden row meets the down matrix as float32, in
-    bfloat16 layers as two bfloat16 terms. An expert or token id out of range sets error bit 1 and is left out."""
+    """A whole expert layer for one to layer.most_tokens tokens (eight, fewer where rows are very wide) in two kernels: routing, the
+    chosen units, the shared unit, the weighted sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the
+    layer's dtype; ids int32 [T] for a layer by table; out float32 (residual itself may be given). Sums are float32; a hidden row meets
+    the down matrix as float32, in bfloat16 layers as the sum of three bfloat16 numbers (24 bits). An expert or token id out of range sets error bit 1 and is left out."""
     T = y.shape[0]
-    if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > MOE_TOKENS:
+    if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > layer.most_tokens:
         raise KernelError(f"moe_tokens: rows {tuple(y.shape)} {y.dtype} do not fit a layer of width {layer.width} {layer.dtype} "
-                          f"(at most {MOE_TOKENS} rows)")
+                          f"(at most {layer.most_tokens} rows)")
     if layer.by_table != (ids is not None) or (ids is not None and (ids.numel() != T or ids.dtype != torch.int32 or not ids.is_contiguous())):
         raise KernelError("moe_tokens: a layer by table wants int32 token ids, one a row, and no other does")
     _check_epilogue("moe_tokens", T, layer.width, None, residual, out)
@@ -1653,14 +1656,14 @@ class Mx4Matrix:
     __slots__ = ("codes", "scales", "width", "shape")
 
     def __init__(self, codes, scales, width):
-        groups = -(-int(width) // MX4_GROUP)
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or width < 1 or codes.dim() < 2 or \
-                codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 64 * groups or scales.shape[-1] != 4 * groups:
+        lead, groups = codes.shape[:-1], (width + MX4_GROUP - 1) // MX4_GROUP
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or width < 1 or not lead or scales.shape != (*lead, 4 * groups) or \
+                codes.shape[-1] != 64 * groups:
             raise KernelError(f"4-bit matrix: codes {tuple(codes.shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} "
                               f"do not fit a width of {width}")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.get_device() != scales.get_device():
             raise KernelError("4-bit matrix: codes and scales must be contiguous and on one device")
-        self.codes, self.scales, self.width, self.shape = codes, scales, int(width), (*codes.shape[:-1], int(width))
+        self.codes, self.scales, self.width, self.shape = codes, scales, width, (*lead, width)
 
     @property
     def device(self):
@@ -1693,7 +1696,8 @@ def mx4_quantize(x):
     _here(x)
     codes = torch.empty((*x.shape[:-1], 64 * groups), dtype=torch.uint8, device=x.device)
     scales = torch.empty((*x.shape[:-1], 4 * groups), dtype=torch.uint8, device=x.device)
-    _call(library("core"), "dd_mx4_quantize", pointer, x.stride(-2), codes.numel() // (64 * groups), x.shape[-1], codes.data_ptr(),
+    # (of a contiguous tensor the stride of a dimension of one may be anything)
+    _call(library("core"), "dd_mx4_quantize", pointer, x.shape[-1] if x.is_contiguous() else x.stride(0), codes.numel() // (64 * groups), x.shape[-1], codes.data_ptr(),
           scales.data_ptr(), dtype, _stream())
     return Mx4Matrix(codes, scales, x.shape[-1])
 
@@ -1711,7 +1715,8 @@ def mx4_values(w, dtype=torch.bfloat16):
 def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, out=None):
     """act(a @ w.T + bias) (+ residual), as gemm_tcgen05 with a 4-bit matrix: a [M, K] bfloat16, w an Mx4Matrix [N, K], bias
     [N] and residual [M, N] float32, out bfloat16 or float32; float32 sums of exact products. Elements of a must be smaller than
-    2^63 in size."""
+    2^63 in size. Beyond MX4_FUSED_ROWS rows the matrix becomes bfloat16 first, which loses nothing (2,048 x 6,400 x 1,600: 36 us,
+    50 for the best of the kernels that turn codes into rows for every tile: they read X once for 128 features)."""
     _rows(a, "a")
     M, K = a.shape
     if a.dtype != torch.bfloat16 or not isinstance(w, Mx4Matrix) or w.dim() != 2 or w.width != K:
@@ -1723,25 +1728,34 @@ def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, ou
     _here(a, w.codes, bias, residual, out)
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    of_bias, of_residual = bias, residual
     bias, residual_stride = _ptr(bias, "bias", torch.float32), 0 if residual is None else residual.stride(0)
     residual = _ptr(residual, "residual", torch.float32)
-    if M > MX4_FEW_ROWS and K % 8 == 0 and a.stride(0) % 8 == 0 and pointer % 16 == 0:
+    if not _mx4_rows(M, N, K) and K % 8 == 0 and a.stride(0) % 8 == 0 and pointer % 16 == 0:
+        if M > MX4_FUSED_ROWS:
+            return gemm_tcgen05(a, mx4_values(w), of_bias, of_residual, activation, out_dtype, out)
         _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), 1, N, None, bias, residual,
-              residual_stride, None, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, 64 if M <= 64 else 128, 0, 0.0, 0.0, 0,
-              ACTIVATIONS[activation], kind, _ptr(error_flag(a.device)), _stream())
+              residual_stride, None, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, 64, 0, 0.0, 0.0, 0,
+              ACTIVATIONS[activation], kind, sm_count(a.device), _ptr(error_flag(a.device)), _stream())
     else:
         _call(library("core"), "dd_gemm_mx4_rows", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), bias, residual,
               residual_stride, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, ACTIVATIONS[activation], kind, _stream())
     return out
 
 
-MX4_FEW_ROWS = 32        # up to here a product streams the matrix through mma.sync; beyond it goes to tcgen05 (rows of whole 16 bytes)
+MX4_FEW_ROWS, MX4_SMALL, MX4_FUSED_ROWS = 32, 1 << 26, 256
+
+
+def _mx4_rows(M, N, K):
+    """Whether a product with a 4-bit matrix streams it through mma.sync (any rows and strides): up to 32 rows, and small
+    products (61 x 1,030 x 1,000 5.0 us, 7.5 on tcgen05; 33 x 1,600 x 6,400 16.1 and 11.5)."""
+    return M <= MX4_FEW_ROWS or M * N * K <= MX4_SMALL
 
 
 def gemm_grouped_mx4(a, w, tile_group, tile, gated=None, out_dtype=None, activation=None, row_scale=None, out=None):
     """gemm_grouped_tcgen05 with a stack of 4-bit matrices (w: an Mx4Matrix [groups, N, K], or [groups, 2 * inner, K] with
     ``gated``): rows of a in tiles that meet one matrix each, with the gated unit or act(row_scale[r] * product) in the epilogue. The
-    rows of a tile whose group is negative are left as they are in ``out``."""
+    rows of a tile whose group is negative are left as they are in ``out``; so are those of a group out of range, which sets error bit 1."""
     _rows(a, "a")
     _check_row_scale(row_scale, a.shape[0])
     if gated and (activation or row_scale is not None):
@@ -1763,7 +1777,7 @@ def gemm_grouped_mx4(a, w, tile_group, tile, gated=None, out_dtype=None, activat
     _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), groups, per_group,
           _ptr(tile_group, "tile_group", torch.int32), None, None, 0, _ptr(row_scale, "row_scale"), _ptr(out, "out", out_dtype), out.stride(0),
           rows, N, K, int(tile), 1 if gated else 0, float(limit), float(alpha), GATED_FORMS[form], ACTIVATIONS[activation], kind,
-          _ptr(error_flag(a.device)), _stream())
+          sm_count(a.device), _ptr(error_flag(a.device)), _stream())
     return out
 
 

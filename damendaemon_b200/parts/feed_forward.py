@@ -42,13 +42,27 @@ def _stacked(runtime, weights, experts, names):
     return _held(runtime, stack)
 
 
+def _check_held(runtime, tensor_cores, width, inner):
+    if runtime.feed_forward == "mx4" and not tensor_cores:
+        raise ValueError(f"experts of {inner} x {width} in 4 bits: both must be multiples of 8 (larger steps run them on the tensor cores)")
+
+
 def _few_tokens(runtime, gate_up, down, **options):
     """The layer as kernels.moe_tokens takes it, or None where the kernels of larger steps serve these too: a runtime that
     wants the kernels whose rows do not depend on what is beside them, float32 matrices of a size whose products keep a row's
     bits for the same reason (splits_float32), or more experts than a block chooses among."""
-    if runtime.gemm == "simt" or (runtime.dtype == torch.float32 and not splits_float32(*down.shape[1:])) or not kernels.expert_layer_fits(options.get("top"), gate_up.shape[0] + options.get("identity", 0) + 1):
+    if runtime.gemm == "simt" or (runtime.dtype == torch.float32 and not splits_float32(*down.shape[1:])) or \
+            not kernels.expert_layer_fits(options["top"], gate_up.shape[0] + options.get("identity", 0) + 1):
         return None
     return kernels.ExpertLayer(gate_up, down, **options)
+
+
+def _runs_few(few, y):
+    """Whether a step of these rows runs a whole expert layer in two kernels (few: _few_tokens). Rows of bfloat16 layers that take more than 48 KB
+    leave its rings too little shared memory (128 experts of 1,536 x 4,096, us with the kernels of larger steps / in two: 4 tokens 268 /
+    218, 8 tokens 390 / 480); float32 layers gain five times either way."""
+    n, width = y.shape
+    return few is not None and n <= few.most_tokens and (y.dtype == torch.float32 or n * width <= 24 << 10)
 
 
 @register_feed_forward("dense")
@@ -121,6 +135,7 @@ class TableRoutedExperts(FeedForward):
             raise ValueError(f"{spec.top} experts per token of {len(spec.experts)}")
         self.table = weights[spec.table]
         self.tensor_cores = grouped_on_tensor_cores(runtime, runtime.dtype, spec.width, first.inner)
+        _check_held(runtime, self.tensor_cores, spec.width, first.inner)
         self.gate_up = _stacked(runtime, weights, spec.experts, lambda u: (u.gate_weight, u.up_weight))
         self.down = _stacked(runtime, weights, spec.experts, lambda u: (u.down_weight,))
         weights[spec.table + ":gate_up"], weights[spec.table + ":down"] = self.gate_up, self.down
@@ -140,7 +155,7 @@ class TableRoutedExperts(FeedForward):
     def forward(self, y, residual, ctx):
         s, rt = self.spec, self.runtime
         unit = s.experts[0]
-        if self.few is not None and y.shape[0] <= kernels.MOE_TOKENS:
+        if _runs_few(self.few, y):
             return kernels.moe_tokens(self.few, y, residual, ids=ctx.token_ids, out=residual)
         if self.shared is not None:
             gate_up = linear(rt, y, self.shared[0])
@@ -250,6 +265,7 @@ class ScoreRoutedExperts(FeedForward):
         self.router = weights[self._router_key(spec)]
         self.correction = weights[spec.correction] if spec.correction else None
         self.tensor_cores = grouped_on_tensor_cores(runtime, runtime.dtype, spec.width, first.inner)
+        _check_held(runtime, self.tensor_cores, spec.width, first.inner)
         # plain units: the up matrices alone
         gates = (lambda u: ()) if self.plain else (lambda u: (u.gate_weight,))
         self.gate_up = _stacked(runtime, weights, spec.experts, lambda u: (*gates(u), u.up_weight))
@@ -300,7 +316,7 @@ class ScoreRoutedExperts(FeedForward):
 
     def forward_terms(self, y, ctx):
         s = self.spec
-        if not s.weight_input or s.shared is not None or (self.few is not None and y.shape[0] <= kernels.MOE_TOKENS):
+        if not s.weight_input or s.shared is not None or _runs_few(self.few, y):
             return super().forward_terms(y, ctx)
         out, pair_row = self._experts(y, *self._route(y)[:2])
         return {"a": out, "pair_row": pair_row}
@@ -314,7 +330,7 @@ class ScoreRoutedExperts(FeedForward):
 
     def forward(self, y, residual, ctx):
         s, rt = self.spec, self.runtime
-        if self.few is not None and y.shape[0] <= kernels.MOE_TOKENS:
+        if _runs_few(self.few, y):
             return kernels.moe_tokens(self.few, y, residual, out=residual)
         chosen, pair_weight, shared_gate = self._route(y)
         if self.shared is not None:

@@ -2,8 +2,8 @@
 
 Tolerance: a product's float32 sum of n terms, in chains of at most n / 8 + 16, is within (n / 8 + 16) 2^-23 of the sum of its terms'
 sizes (the tensor cores cut off where they add). The hidden rows' own error goes through the down product: with slope 2 at most for the units
-at these sizes (|gate|, |up| below 4), relative to the sum of sizes of the up products; two bfloat16 terms keep 2^-17 of a hidden
-value. Every bound below is that sum of sizes, computed beside the result."""
+at these sizes (|gate|, |up| below 4), relative to the sum of sizes of the up products; the bfloat16 terms of a hidden value
+(two would do) keep 2^-17 of it. Every bound below is that sum of sizes, computed beside the result."""
 import pytest
 import torch
 

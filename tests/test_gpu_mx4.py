@@ -85,6 +85,8 @@ def test_quantize_strided_stacked_and_again():
     odd = x[:, 3:100]                                        # rows that start between 16-byte boundaries
     assert torch.equal(kernels.mx4_quantize(odd).codes, kernels.mx4_quantize(odd.contiguous()).codes)
     stack = randn(6, 3, 5, 96).to(DEV)
+    single = stack[:, 0].contiguous().as_strided((3, 1, 96), (96, 1 << 20, 1))      # contiguous: a dimension of one has any stride
+    assert torch.equal(kernels.mx4_quantize(single).codes, kernels.mx4_quantize(stack[:, :1].contiguous()).codes)
     q = kernels.mx4_quantize(stack)
     assert q.shape == (3, 5, 96)
     assert torch.equal(q.codes[1], kernels.mx4_quantize(stack[1]).codes)
@@ -100,8 +102,17 @@ SHAPES = [(1, 16, 32), (1, 1, 1), (2, 17, 100), (3, 130, 128), (7, 33, 129), (8,
           (129, 384, 72), (257, 130, 1024), (300, 64, 33)]
 
 
-@pytest.mark.parametrize("M,N,K", SHAPES)
-def test_gemm_mx4(M, N, K):
+@pytest.fixture(params=["rule", "tcgen05", "unpacked"])
+def path(request, monkeypatch):
+    """The kernel that the sizes choose; tcgen05 wherever it can run; the matrix turned into bfloat16 wherever it can."""
+    if request.param != "rule":
+        monkeypatch.setattr(kernels, "MX4_SMALL", 0)
+        monkeypatch.setattr(kernels, "MX4_FEW_ROWS", 0)
+        monkeypatch.setattr(kernels, "MX4_FUSED_ROWS", 1 << 30 if request.param == "tcgen05" else 0)
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES + [(300, 1100, 520), (64, 1600, 6400), (260, 2048, 1024)])
+def test_gemm_mx4(path, M, N, K):
     a, w = randn(M + K, M, K, dtype=torch.bfloat16), randn(N + K, N, K, scale=K ** -0.5)
     q = kernels.mx4_quantize(w.to(DEV))
     values = kernels.mx4_values(q, torch.float32).double().cpu()
@@ -112,7 +123,7 @@ def test_gemm_mx4(M, N, K):
 
 @pytest.mark.parametrize("M,N,K", [(1, 33, 100), (8, 64, 256), (20, 130, 384), (70, 130, 264), (200, 100, 1000)])
 @pytest.mark.parametrize("act", [None, "gelu_new", "gelu", "relu2", "tanh"])
-def test_gemm_mx4_epilogue(M, N, K, act):
+def test_gemm_mx4_epilogue(path, M, N, K, act):
     a, w = randn(M, M, K, dtype=torch.bfloat16), randn(N, N, K, scale=K ** -0.5)
     bias, residual = randn(1, N), randn(2, M, N)
     q = kernels.mx4_quantize(w.to(DEV))
@@ -129,13 +140,15 @@ def test_gemm_mx4_epilogue(M, N, K, act):
     close(kernels.gemm_mx4(a.to(DEV), q, bias.to(DEV), residual.to(DEV), act), want, bound)
 
 
-def test_gemm_mx4_strides_and_rows_beside():
+def test_gemm_mx4_strides_and_rows_beside(path):
     a, w = randn(3, 12, 600, dtype=torch.bfloat16).to(DEV), randn(4, 50, 200, scale=0.1).to(DEV)
     q = kernels.mx4_quantize(w)
+    values = kernels.mx4_values(q, torch.float32).double().cpu()
     for part in (a[:, 200:400], a[:, 3:203], a[1:, 400:], a[::2, :200]):
         store = torch.full((part.shape[0], 70), 7.0, device=DEV)
         got = kernels.gemm_mx4(part, q, out_dtype=torch.float32, out=store[:, 5:55])
-        assert torch.equal(got, kernels.gemm_mx4(part.contiguous(), q, out_dtype=torch.float32))
+        # (rows that are no whole 16-byte pieces go through mma.sync whatever the path: not the same order of summing)
+        close(got, part.double().cpu() @ values.t(), product_bound(part.cpu(), values))
         assert (store[:, :5] == 7).all() and (store[:, 55:] == 7).all()
     many = randn(8, 150, 200, dtype=torch.bfloat16).to(DEV)
     store = torch.full((152, 50), 7.0, device=DEV)
@@ -144,7 +157,7 @@ def test_gemm_mx4_strides_and_rows_beside():
 
 
 @pytest.mark.parametrize("M", [1, 8, 40, 140])
-def test_gemm_mx4_wide_scales(M):
+def test_gemm_mx4_wide_scales(path, M):
     """Blocks whose scales lie far apart, weights above and below 1, large and small rows of a."""
     K = 512
     w = randn(1, 48, K) * torch.exp2(torch.randint(-40, 41, (48, K // 32), generator=torch.Generator().manual_seed(2)).repeat_interleave(32, 1).float())
@@ -155,7 +168,7 @@ def test_gemm_mx4_wide_scales(M):
 
 
 @pytest.mark.parametrize("M", [2, 70])
-def test_gemm_mx4_not_finite(M):
+def test_gemm_mx4_not_finite(path, M):
     w, a = randn(1, 40, 160), randn(2, M, 160, dtype=torch.bfloat16)
     w[5, 70] = float("nan")
     a[1, 9] = float("inf")
@@ -171,10 +184,10 @@ def test_gemm_mx4_no_rows():
     assert kernels.gemm_mx4(torch.empty((0, 160), dtype=torch.bfloat16, device=DEV), q).shape == (0, 40)
 
 
-def test_gemm_mx4_replayed():
+def test_gemm_mx4_replayed(path):
     """Captured once, replayed with other inputs, while the same call runs outside the graph."""
     q = kernels.mx4_quantize(randn(1, 200, 320).to(DEV))
-    for M in (4, 90):
+    for M in (4, 90, 300):
         a = randn(M, M, 320, dtype=torch.bfloat16).to(DEV)
         kernels.gemm_mx4(a, q)
         torch.cuda.synchronize()
@@ -237,6 +250,47 @@ def test_grouped_gated(tile, inner, K, form):
             want = gated(gate, up, 2.0, 1.702, form)
             # the unit's slopes: at most 1.13 (|up| + 1) by the gate, |gate| + 1 by up; its exponential is the special-function unit's, 2^-20
             close(got[part], want, 1.13 * (up.abs() + 1) * bg + (gate.abs() + 1) * bu + 2.0 ** -18 * (want.abs() + gate.abs()))
+
+
+@pytest.mark.parametrize("N,K,tiles", [(2500, 200, 10), (130, 72, 90), (1300, 1024, 16)])
+def test_grouped_with_more_tiles_than_sms(N, K, tiles):
+    """Tiles of 128 rows that a block takes one after the other, some of them without rows, at either end and in between."""
+    g = torch.Generator().manual_seed(N)
+    groups = torch.randint(-1, 3, (tiles,), generator=g).tolist()
+    groups[0], groups[-1] = -1, 2
+    a, w = randn(N, 128 * tiles, K, dtype=torch.bfloat16), randn(K, 3, N, K, scale=K ** -0.5)
+    scale = randn(7, 128 * tiles).abs()
+    q = kernels.mx4_quantize(w.to(DEV))
+    values = kernels.mx4_values(q, torch.float32).double().cpu()
+    which = torch.tensor(groups, dtype=torch.int32, device=DEV)
+    for dtype, by, act in ((torch.float32, None, None), (torch.bfloat16, scale, "relu2")):
+        out = torch.full((128 * tiles, N), 7.0, dtype=dtype, device=DEV)
+        kernels.gemm_grouped_mx4(a.to(DEV), q, which, 128, activation=act, row_scale=None if by is None else by.to(DEV), out=out)
+        for i, e in enumerate(groups):
+            part = slice(128 * i, 128 * (i + 1))
+            if e < 0:
+                assert (out[part] == 7).all()
+                continue
+            f = 1.0 if by is None else by[part].double().unsqueeze(1)
+            z = a[part].double() @ values[e].t() * f
+            want = activation(z, act)
+            slope = 2 * z.abs() + 1 if act else 1.0
+            close(out[part], want, product_bound(a[part], values[e], 1) * f * slope + 2.0 ** -20 * (z.abs() + want.abs()))
+
+
+@pytest.mark.parametrize("tile,tiles,gated", [(16, 3, None), (128, 3, None), (128, 200, None), (64, 3, (1.0, 1.0, "silu"))])
+def test_grouped_without_such_a_matrix(tile, tiles, gated):
+    """A group out of range is an error that the device reports; its rows stay, the others are computed."""
+    q = kernels.mx4_quantize(randn(1, 2, 130, 64).to(DEV))
+    a = randn(2, tile * tiles, 64, dtype=torch.bfloat16).to(DEV)
+    which = torch.ones(tiles, dtype=torch.int32, device=DEV)
+    want = kernels.gemm_grouped_mx4(a, q, which, tile, gated)
+    assert kernels.read_error_flag(DEV) == 0
+    which[1] = 2
+    out = torch.full_like(want, 7.0)
+    kernels.gemm_grouped_mx4(a, q, which, tile, gated, out=out)
+    assert kernels.read_error_flag(DEV) == 1
+    assert (out[tile:2 * tile] == 7).all() and torch.equal(out[:tile], want[:tile]) and torch.equal(out[2 * tile:], want[2 * tile:])
 
 
 def test_grouped_refusals():
