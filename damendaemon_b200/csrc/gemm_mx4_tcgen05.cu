@@ -53,9 +53,9 @@ template <int T, bool DUAL, bool SPLIT = false> struct Mx4Config {
     static constexpr int DEQUANT_WARPS = 4 * SETS, THREADS = (DEQUANT_WARPS + 2) * 32;
     static constexpr int X_BYTES = T * XK * 2;
     static constexpr int W_BYTES = (DUAL ? 2 : 1) * CODE_BYTES;
-    static constexpr int W_STAGES = DUAL ? 2 : 2 * SETS;             // (a set always meets the same stages: see the rings)
+    static constexpr int W_STAGES = 4;                               // (a set always meets the same stages: see the rings)
     static constexpr int ACC_COLS = (DUAL ? 2 : 1) * T;
-    static constexpr int A_STAGES = DUAL ? 2 : 2 * SETS;             // of 32 columns (64 k), twice that with DUAL
+    static constexpr int A_STAGES = DUAL ? (T <= 32 ? 3 : 2) : 2 * SETS;      // of 32 columns (64 k), twice that with DUAL
     static constexpr int A_COLS = A_STAGES * (DUAL ? 64 : 32);
     static constexpr int TMEM_COLS = ACC_COLS + A_COLS <= 256 ? 256 : 512;
     static constexpr int BLOCKS = TMEM_COLS == 256 ? 2 : 1;          // an SM
@@ -243,11 +243,12 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const uint32_t* scales = p.scales + w_row * p.k_groups + k_first;
             constexpr int STEP = DUAL ? 1 : SETS;
             const int first = DUAL ? 0 : set;
-            uint32_t four = first < kgroups ? scales[first] : 0u;
+            uint32_t four = first < kgroups ? scales[first] : 0u, next = first + STEP < kgroups ? scales[first + STEP] : 0u;
             bool ok = true;
             for (int i = first; i < kgroups && ok; i += STEP) {
                 const uint32_t by = four;
-                if (i + STEP < kgroups) four = scales[i + STEP];
+                four = next;
+                if (i + 2 * STEP < kgroups) next = scales[i + 2 * STEP];
                 const int s = i % C::W_STAGES;
                 if (!tc::mbar_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
                 uint32_t words[4][4];

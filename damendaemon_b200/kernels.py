@@ -1656,9 +1656,9 @@ class Mx4Matrix:
     __slots__ = ("codes", "scales", "width", "shape")
 
     def __init__(self, codes, scales, width):
-        lead, groups = codes.shape[:-1], (width + MX4_GROUP - 1) // MX4_GROUP
+        (*lead, wide), groups = codes.shape, (width + MX4_GROUP - 1) // MX4_GROUP
         if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or width < 1 or not lead or scales.shape != (*lead, 4 * groups) or \
-                codes.shape[-1] != 64 * groups:
+                wide != 64 * groups:
             raise KernelError(f"4-bit matrix: codes {tuple(codes.shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} "
                               f"do not fit a width of {width}")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.get_device() != scales.get_device():
@@ -1685,21 +1685,28 @@ def _here(*tensors):
             raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{current}")
 
 
+def _like(t, shape, dtype):
+    """An empty tensor beside another one (of its type new_empty makes it in 1.6 us, torch.empty in 2.6)."""
+    return t.new_empty(shape) if t.dtype is dtype else torch.empty(shape, dtype=dtype, device=t.device)
+
+
 def mx4_quantize(x):
     """x [..., rows, width] float32 or bfloat16 -> Mx4Matrix: per block of 32 the power of two that brings its largest element
     into [4, 8), every element rounded to the nearest number, ties to the even one, sizes above 6 to 6. A block with an
     infinity or a NaN has no values (they read as NaN, and products with it are not finite). Rows may have a stride if x is 2-D."""
-    if x.dim() < 2 or x.shape[-1] < 1 or (not x.is_contiguous() and (x.dim() != 2 or x.stride(1) != 1)):
+    contiguous = x.is_contiguous()
+    if x.dim() < 2 or x.shape[-1] < 1 or (not contiguous and (x.dim() != 2 or x.stride(1) != 1)):
         raise KernelError(f"mx4_quantize: rows of contiguous elements wanted, got shape {tuple(x.shape)} strides {x.stride()}")
-    groups = -(-x.shape[-1] // MX4_GROUP)
+    *lead, width = x.shape
+    groups = -(-width // MX4_GROUP)
     pointer, dtype = _ptr(x, "x"), _dt(x.dtype)
     _here(x)
-    codes = torch.empty((*x.shape[:-1], 64 * groups), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], 4 * groups), dtype=torch.uint8, device=x.device)
+    codes = torch.empty((*lead, 64 * groups), dtype=torch.uint8, device=x.device)
+    scales = codes.new_empty((*lead, 4 * groups))
     # (of a contiguous tensor the stride of a dimension of one may be anything)
-    _call(library("core"), "dd_mx4_quantize", pointer, x.shape[-1] if x.is_contiguous() else x.stride(0), codes.numel() // (64 * groups), x.shape[-1], codes.data_ptr(),
+    _call(library("core"), "dd_mx4_quantize", pointer, width if contiguous else x.stride(0), x.numel() // width, width, codes.data_ptr(),
           scales.data_ptr(), dtype, _stream())
-    return Mx4Matrix(codes, scales, x.shape[-1])
+    return Mx4Matrix(codes, scales, width)
 
 
 def mx4_values(w, dtype=torch.bfloat16):
@@ -1707,8 +1714,7 @@ def mx4_values(w, dtype=torch.bfloat16):
     pointer, kind = _ptr(w.codes, "codes"), _dt(dtype)
     _here(w.codes)
     out = torch.empty(w.shape, dtype=dtype, device=w.device)
-    _call(library("core"), "dd_mx4_values", pointer, w.scales.data_ptr(), w.scales.numel() // w.scales.shape[-1], w.width, out.data_ptr(),
-          kind, _stream())
+    _call(library("core"), "dd_mx4_values", pointer, w.scales.data_ptr(), out.numel() // w.width, w.width, out.data_ptr(), kind, _stream())
     return out
 
 
@@ -1722,12 +1728,13 @@ def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, ou
     if a.dtype != torch.bfloat16 or not isinstance(w, Mx4Matrix) or w.dim() != 2 or w.width != K:
         raise KernelError(f"gemm_mx4: needs bfloat16 a [M, K] and a 4-bit matrix [N, K]; got {tuple(a.shape)} {a.dtype}, {tuple(w.shape)}")
     N = w.shape[0]
-    _check_epilogue("gemm_mx4", M, N, bias, residual, out)
+    if bias is not None or residual is not None or out is not None:
+        _check_epilogue("gemm_mx4", M, N, bias, residual, out)
     out_dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
     kind, pointer = _dt(out_dtype), _ptr(a, "a")
     _here(a, w.codes, bias, residual, out)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+        out = _like(a, (M, N), out_dtype)
     of_bias, of_residual = bias, residual
     bias, residual_stride = _ptr(bias, "bias", torch.float32), 0 if residual is None else residual.stride(0)
     residual = _ptr(residual, "residual", torch.float32)
