@@ -192,24 +192,23 @@ __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0,
         }
     } else {
         // (the tensor cores cut off where they add: a sum of 64 products starts from nothing and is added rounded)
-        uint4 a[2][2];
+        float e[P][4];
+#pragma unroll
+        for (int p = 0; p < P; ++p) e[p][0] = e[p][1] = e[p][2] = e[p][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t at = slot + g * 128 + ((2 * t + i) ^ g) * 16;
-            a[i][0] = few::lds16(at);
-            a[i][1] = few::lds16(at + 1024);
-        }
+            const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            float e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                few::mma(e, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b[p][i].x, b[p][i].y);
-                few::mma(e, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b[p][i].z, b[p][i].w);
+            for (int p = 0; p < P; ++p) {
+                few::mma(e[p], a0.x, a1.x, a0.y, a1.y, b[p][i].x, b[p][i].y);
+                few::mma(e[p], a0.z, a1.z, a0.w, a1.w, b[p][i].z, b[p][i].w);
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[p][j] += e[j];
         }
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[p][j] += e[p][j];
     }
 }
 __device__ __forceinline__ void put_tile(Tile& to, const float* d, float by = 1.f) {
