@@ -37,6 +37,7 @@ struct Mx4Params {
     int* error_flag;
     int rows, N, K, k_groups, groups, rows_per_group, ldr, ldo, out_dtype, act, form;
     float limit, alpha;
+    mx4::Shifts shifts;
 };
 
 // The matrix of a tile of rows, or -1: skipped on purpose, or no such matrix (an error, and nothing is read or written).
@@ -96,13 +97,13 @@ __device__ __forceinline__ void read_codes(const uint8_t* tile, int row, uint32_
     }
 }
 // Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales.
-__device__ __forceinline__ void half_of(const uint32_t (*words)[4], uint32_t four, int half, uint32_t* r) {
+__device__ __forceinline__ void half_of(const uint32_t (*words)[4], const mx4::Shifts& shifts, uint32_t four, int half, uint32_t* r) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         const uint32_t scale = (four >> (16 * half + 8 * b)) & 255u, factor = pair_factor(scale);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            mx4::pairs(words[t][2 * half + b], r + b * 16 + t * 4);
+            mx4::pairs(words[t][2 * half + b], shifts, r + b * 16 + t * 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor);
         }
@@ -260,7 +261,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     const int h = 2 * i + half, a = h % C::A_STAGES;
                     if (h >= kblocks) break;
                     uint32_t r[32];
-                    half_of(words, by, half, r);
+                    half_of(words, p.shifts, by, half, r);
                     if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
                     tc::tmem_st_x32(tmem_a + lane_part + a * (DUAL ? 64 : 32) + (DUAL ? set * 32 : 0), r);
@@ -456,7 +457,7 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 for (int half = 0; half < 2; ++half) {
                     const int h = h0 + 2 * i + half, a = h % C::A_STAGES;
                     uint32_t r[32];
-                    half_of(words, by, half, r);
+                    half_of(words, p.shifts, by, half, r);
                     if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
                     tc::tmem_st_x32(tmem_a + lane_part + a * 32, r);
@@ -584,7 +585,7 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
     Mx4Params p;
     p.scales = (const uint32_t*)scales; p.tile_group = tile_group; p.bias = bias; p.residual = residual; p.row_scale = row_scale; p.out = out;
     p.error_flag = error_flag; p.rows = rows; p.N = N; p.K = K; p.k_groups = dd_ceil_div(K, mx4::GROUP); p.groups = groups; p.rows_per_group = rows_per_group;
-    p.ldr = ldr; p.ldo = ldo; p.out_dtype = out_dtype; p.act = act; p.form = form; p.limit = limit; p.alpha = alpha;
+    p.ldr = ldr; p.ldo = ldo; p.out_dtype = out_dtype; p.act = act; p.form = form; p.limit = limit; p.alpha = alpha; p.shifts = mx4::SHIFTS;
     const long long row_bytes = (long long)p.k_groups * mx4::GROUP_BYTES;
     CUtensorMap mw, mx;
     if (int e = mx4_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, (long long)groups * rows_per_group, row_bytes, row_bytes, mx4::GROUP_BYTES, BM,

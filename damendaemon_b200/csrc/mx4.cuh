@@ -21,6 +21,17 @@ __device__ __forceinline__ void pairs(uint32_t w, uint32_t* v) {
     v[2] = ((w << 4) & SIGN) | ((w >> 2) & SIZE);
     v[3] = (w & SIGN) | ((w >> 6) & SIZE);
 }
+// The same with multiplications for the shifts to the left: masks and multiply-adds then take two pipes by turns. The powers of two come
+// from the launch (a constant would be made a shift again).
+struct Shifts { uint32_t by4, by16, by64, by256, by4096; };
+constexpr Shifts SHIFTS = {4, 16, 64, 256, 4096};
+__device__ __forceinline__ void pairs(uint32_t w, const Shifts& m, uint32_t* v) {
+    const uint32_t down = w >> 6;
+    v[0] = (w & 0x00080008u) * m.by4096 + (w & 0x00070007u) * m.by64;
+    v[1] = (w & 0x00800080u) * m.by256 + (w & 0x00700070u) * m.by4;
+    v[2] = ((w & 0x08000800u) | (down & 0x001C001Cu)) * m.by16;
+    v[3] = (w & 0x80008000u) | (down & 0x01C001C0u);
+}
 // The eight elements of a word as float16 pairs (0,2) (4,6) (1,3) (5,7), one instruction a pair. (83 elements a clock and SM, the
 // bfloat16 pairs above 45.)
 __device__ __forceinline__ void pairs_f16(uint32_t w, uint32_t* v) {
