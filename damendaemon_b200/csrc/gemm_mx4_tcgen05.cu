@@ -2,7 +2,7 @@
 //
 //     out[r, n] = act(scale[r] * sum_k X[r, k] W[group(tile of r)][n, k] + bias[n]) (+ residual[r, n])
 //
-// X bfloat16 in row tiles, W one matrix or a stack of them of which a tile meets one; or, DUAL, the gated unit of two such products
+// X bfloat16 in row tiles, W one matrix or a stack of them of which a tile meets one; or, PAIRED, the gated unit of two such products
 // (N gate rows, then N up rows a group), as gemm_grouped_tcgen05.cu does it for bfloat16 matrices.
 //
 // An element times its block's scale is a bfloat16 number exactly, so the weights become bfloat16 on their way to the tensor
@@ -14,10 +14,17 @@
 // these kernels cost beside a bfloat16 product; they are for rows that meet different matrices (grouped by expert) and for up to a few
 // hundred rows, where it hides behind the codes' way from memory.
 //
-// Rings: X (64 k a stage, TMA -> MMA), codes (128 k, TMA -> the eight warps), W in tensor memory (64 k, warps -> MMA). Without DUAL
-// the two sets of four warps take groups of 128 k in turn, with it one set the gate's and one the up rows. Sets that take turns need rings
-// whose length they divide, so that a stage's phases are all waited for by one of them: a wait for the phase after one that has not
-// ended yet passes at once. Every wait is bounded.
+// The gated unit (PAIRED): a block has 64 features, and the lanes of the accumulator are gate rows and up rows by turns of sixteen, so that
+// a gate value and its up value meet by one exchange within a warp. (As two accumulators of 128 features each, the sets of
+// warps taking the gate's and the up rows: 26.7 us instead of 22.8 for 17 tiles of 16 rows of 3,200 x 1,600, 24.9 and 14.9 for 11: half
+// as many blocks of twice the length.)
+//
+// Rings: X (64 k a stage, TMA -> MMA), codes (128 k, TMA -> the eight warps), W in tensor memory (64 k, warps -> MMA). The two sets of
+// four warps take groups of 128 k in turn. Sets that take turns need stages whose phases they cannot miss, since a wait for the phase
+// after one that has not ended yet passes at once: codes lie in rings whose length the sets divide, so that a stage is always one
+// set's; so does W in its ring of four, and in its ring of three a set that turns to half h (of 64 k) has waited for the products of half h - 6
+// already (its half before that was h - 1 or h - 3, which waited for h - 4 or h - 6), so the phase it asks for is the present one or past. Every wait is
+// bounded, and a warp's lanes decide alike.
 #include "common.cuh"
 #include "mx4.cuh"
 #include "tcgen05.cuh"
@@ -49,23 +56,23 @@ __device__ __forceinline__ int matrix_of(const Mx4Params& p, int tile) {
 }
 
 // SPLIT: the blocks of a cluster share K (tiles of 64 rows that are too few for the GPU otherwise).
-template <int T, bool DUAL, bool SPLIT = false> struct Mx4Config {
+template <int T, bool SPLIT = false> struct Mx4Config {
     static constexpr int SETS = 2;                                   // of four warps that turn codes into rows
     static constexpr int DEQUANT_WARPS = 4 * SETS, THREADS = (DEQUANT_WARPS + 2) * 32;
     static constexpr int X_BYTES = T * XK * 2;
-    static constexpr int W_BYTES = (DUAL ? 2 : 1) * CODE_BYTES;
+    static constexpr int W_BYTES = CODE_BYTES;
     static constexpr int W_STAGES = 4;                               // (a set always meets the same stages: see the rings)
-    static constexpr int ACC_COLS = (DUAL ? 2 : 1) * T;
-    static constexpr int A_STAGES = DUAL ? (T <= 32 ? 3 : 2) : 2 * SETS;      // of 32 columns (64 k), twice that with DUAL
-    static constexpr int A_COLS = A_STAGES * (DUAL ? 64 : 32);
-    static constexpr int TMEM_COLS = ACC_COLS + A_COLS <= 256 ? 256 : 512;
-    static constexpr int BLOCKS = TMEM_COLS == 256 ? 2 : 1;          // an SM
+    static constexpr int ACC_COLS = T;
+    static constexpr int A_STAGES = T <= 32 ? 3 : 4;                 // of 32 columns (64 k)
+    static constexpr int A_COLS = A_STAGES * 32;
+    static constexpr int TMEM_COLS = ACC_COLS + A_COLS <= 128 ? 128 : 256;
+    static constexpr int BLOCKS = TMEM_COLS == 128 ? 3 : 2;          // an SM
     static constexpr int RED_BYTES = SPLIT ? BM * T * 4 : 0;         // the cluster's partial sums of this block's columns
-    static constexpr int X_FIT = ((BLOCKS == 2 ? 108 : 216) * 1024 - W_STAGES * W_BYTES - RED_BYTES) / X_BYTES;
+    static constexpr int X_FIT = ((BLOCKS == 2 ? 108 : 72) * 1024 - W_STAGES * W_BYTES - RED_BYTES) / X_BYTES;
     static constexpr int X_STAGES = X_FIT < 8 ? X_FIT : 8;
     static constexpr int BARRIERS = 2 * (X_STAGES + W_STAGES + A_STAGES) + 1;
     static constexpr int SMEM_BYTES = X_STAGES * X_BYTES + W_STAGES * W_BYTES + RED_BYTES + 1024 + BARRIERS * 8 + 16;
-    static_assert((DUAL || (W_STAGES % SETS == 0 && A_STAGES % (2 * SETS) == 0)) && ACC_COLS + A_COLS <= 512 && SMEM_BYTES <= 227 * 1024, "tensor or shared memory");
+    static_assert(W_STAGES % SETS == 0 && ACC_COLS + A_COLS <= TMEM_COLS && SMEM_BYTES <= 227 * 1024, "tensor or shared memory");
 };
 
 __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
@@ -83,6 +90,11 @@ __device__ __forceinline__ uint32_t pair_factor(uint32_t s) {
     return bits | (bits << 16);
 }
 
+// A wait by all lanes of a warp: they decide alike.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
+}
+
 template <int A> struct Act { static constexpr int value = A; };
 template <typename T> struct As { using Type = T; };
 
@@ -96,37 +108,50 @@ __device__ __forceinline__ void read_codes(const uint8_t* tile, int row, uint32_
         words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
     }
 }
-// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales.
+// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales. Scales of 1 .. 128 (all blocks but those of zeros and those whose largest
+// element passes 16) need no case of their own.
 __device__ __forceinline__ void half_of(const uint32_t (*words)[4], const mx4::Shifts& shifts, uint32_t four, int half, uint32_t* r) {
+    const bool easy = ((four - 0x01010101u) & 0x80808080u) == 0;
+    uint32_t scale[2], factor[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const uint32_t scale = (four >> (16 * half + 8 * b)) & 255u, factor = pair_factor(scale);
+        scale[b] = (four >> (16 * half + 8 * b)) & 255u;
+        factor[b] = scale[b] * 0x00800080u + 0x3F003F00u;                    // pair_factor(scale[b])
+    }
+    if (!easy) {
+        factor[0] = pair_factor(scale[0]);
+        factor[1] = pair_factor(scale[1]);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             mx4::pairs(words[t][2 * half + b], shifts, r + b * 16 + t * 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor);
+            for (int j = 0; j < 4; ++j) r[b * 16 + t * 4 + j] = mul_pair(r[b * 16 + t * 4 + j], factor[b]);
         }
-        if (scale > 128 && scale < 255) {
-            const uint32_t more = ((scale - 1) << 7) * 0x10001u;             // 2^(s - 128)
+    if (!easy)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) r[b * 16 + j] = mul_pair(r[b * 16 + j], more);
-        }
-    }
+        for (int b = 0; b < 2; ++b)
+            if (scale[b] > 128 && scale[b] < 255) {
+                const uint32_t more = ((scale[b] - 1) << 7) * 0x10001u;      // 2^(s - 128)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) r[b * 16 + j] = mul_pair(r[b * 16 + j], more);
+            }
 }
-// Results of feature n, rows r .. r + count - 1 (at most eight), from their sums; what the product's epilogue has is chosen outside of the
+// Results of feature n, rows r .. r + count - 1 (at most MOST), from their sums; what the product's epilogue has is chosen outside of the
 // loop over them.
-template <bool DUAL>
+template <bool PAIRED, int MOST = 8>
 __device__ __forceinline__ void finish(const Mx4Params& p, int n, float bias, int r, int count, const float* g, const float* u) {
     auto columns = [&](auto act, auto type) {
         using Out = typename decltype(type)::Type;
         Out* out = reinterpret_cast<Out*>(p.out) + (size_t)r * p.ldo + n;
         const float* residual = p.residual ? p.residual + (size_t)r * p.ldr + n : nullptr;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < MOST; ++j) {
             if (j >= count) break;
             float v = g[j];
-            if (DUAL) v = dd_gated_value<true>(v, u[j], p.form, p.limit, p.alpha);
+            if (PAIRED) v = dd_gated_value<true>(v, u[j], p.form, p.limit, p.alpha);
             else {
                 if (p.row_scale) v *= p.row_scale[r + j];
                 v += bias;
@@ -146,10 +171,43 @@ __device__ __forceinline__ void finish(const Mx4Params& p, int n, float bias, in
     else columns(Act<DD_ACT_TANH>{}, As<float>{});
 }
 
-template <int T, bool DUAL, bool SPLIT>
-__global__ void __launch_bounds__((Mx4Config<T, DUAL, SPLIT>::THREADS), (Mx4Config<T, DUAL, SPLIT>::BLOCKS))
+// The features of a block, and where a thread finds its own: lane `quarter * 32 + lane` of the accumulator is that feature's row, or, PAIRED, lanes
+// 0 .. 15 of a quarter are the gate rows of sixteen features and 16 .. 31 their up rows (in the stage: 64 gate rows, then 64 up rows).
+template <bool PAIRED> constexpr int features = PAIRED ? BM / 2 : BM;
+struct Place {
+    int feature, staged;
+    bool up;
+    __device__ __forceinline__ Place(int quarter, int lane, bool paired) {
+        up = paired && lane >= 16;
+        feature = paired ? quarter * 16 + (lane & 15) : quarter * 32 + lane;
+        staged = feature + (up ? BM / 2 : 0);
+    }
+};
+__device__ __forceinline__ size_t matrix_row(const Mx4Params& p, int group, int n0, const Place& at) {
+    return (size_t)group * p.rows_per_group + (at.up ? p.N : 0) + min(n0 + at.feature, p.N - 1);
+}
+// The results of a lane's eight columns, rows r .. r + count - 1. PAIRED: a gate lane and its up lane exchange halves, and finish four
+// rows each.
+template <bool PAIRED>
+__device__ __forceinline__ void finish_eight(const Mx4Params& p, int n, bool live, float bias, int r, int count, const float* v) {
+    if (PAIRED) {
+        const bool up = threadIdx.x & 16;
+        float g[4], u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[4 + j], 16);
+            g[j] = up ? other : v[j];
+            u[j] = up ? v[4 + j] : other;
+        }
+        if (live) finish<true, 4>(p, n, 0.f, up ? r + 4 : r, up ? count - 4 : count, g, u);
+    } else if (live)
+        finish<false>(p, n, bias, r, count, v, nullptr);
+}
+
+template <int T, bool PAIRED, bool SPLIT>
+__global__ void __launch_bounds__((Mx4Config<T, SPLIT>::THREADS), (Mx4Config<T, SPLIT>::BLOCKS))
 gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Mx4Params p) {
-    using C = Mx4Config<T, DUAL, SPLIT>;
+    using C = Mx4Config<T, SPLIT>;
     constexpr int DEQUANT_WARPS = C::DEQUANT_WARPS, SETS = C::SETS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* x_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -168,8 +226,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::X_STAGES; ++s) { tc::mbar_init(&x_full[s], 1); tc::mbar_init(&x_empty[s], 1); }
-        for (int s = 0; s < C::W_STAGES; ++s) { tc::mbar_init(&w_full[s], 1); tc::mbar_init(&w_empty[s], DUAL ? 8 : 4); }
-        for (int s = 0; s < C::A_STAGES; ++s) { tc::mbar_init(&a_full[s], DUAL ? 8 : 4); tc::mbar_init(&a_empty[s], 1); }
+        for (int s = 0; s < C::W_STAGES; ++s) { tc::mbar_init(&w_full[s], 1); tc::mbar_init(&w_empty[s], 4); }
+        for (int s = 0; s < C::A_STAGES; ++s) { tc::mbar_init(&a_full[s], 4); tc::mbar_init(&a_empty[s], 1); }
         tc::mbar_init(acc_bar, 1);
         *abort_flag = 0;
         tc::fence_barrier_init();
@@ -188,7 +246,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     dd_grid_wait();              // the tile's group and the rows are earlier kernels' results
 
     const int splits = SPLIT ? (int)tc::cluster_size() : 1, rank = SPLIT ? (int)tc::cluster_rank() : 0;
-    const int n0 = blockIdx.x / splits * BM, row0 = blockIdx.y * T;
+    const int n0 = blockIdx.x / splits * features<PAIRED>, row0 = blockIdx.y * T;
     const int group = matrix_of(p, blockIdx.y);
     // this block's groups of 128 k, and its blocks of 64 (h counts from the first of them)
     const int k_first = p.k_groups * rank / splits, kgroups = p.k_groups * (rank + 1) / splits - k_first;
@@ -205,7 +263,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     if (!tc::mbar_wait(&w_empty[s], ((i / C::W_STAGES) & 1) ^ 1, abort_flag)) break;
                     tc::mbar_expect_tx(&w_full[s], C::W_BYTES);
                     tc::tma_load_2d(w_tiles + s * C::W_BYTES, &map_w, (k_first + i) * mx4::GROUP_BYTES, w_row, &w_full[s]);
-                    if (DUAL) tc::tma_load_2d(w_tiles + s * C::W_BYTES + CODE_BYTES, &map_w, (k_first + i) * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
+                    if (PAIRED) tc::tma_load_2d(w_tiles + s * C::W_BYTES + CODE_BYTES / 2, &map_w, (k_first + i) * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
                     for (int h = 2 * i; h < min(2 * i + 2, kblocks); ++h) {
                         const int x = h % C::X_STAGES;
                         if (!tc::mbar_wait(&x_empty[x], ((h / C::X_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -224,12 +282,11 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                         !tc::mbar_wait(&a_full[a], (h / C::A_STAGES) & 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
                     const uint32_t x_addr = tc::smem_u32(x_tiles + x * C::X_BYTES);
-                    const uint32_t from = tmem_a + a * (DUAL ? 64 : 32);
+                    const uint32_t from = tmem_a + a * 32;
 #pragma unroll
                     for (int k = 0; k < XK / UMMA_K; ++k) {
                         const uint64_t dx = tc::smem_desc_sw128(x_addr + k * UMMA_K * 2);
                         tc::mma_bf16_a_tmem(tmem, from + k * (UMMA_K / 2), dx, idesc, (h > 0 || k > 0) ? 1u : 0u);
-                        if (DUAL) tc::mma_bf16_a_tmem(tmem + T, from + 32 + k * (UMMA_K / 2), dx, idesc, (h > 0 || k > 0) ? 1u : 0u);
                     }
                     tc::mma_commit(&x_empty[x]);
                     tc::mma_commit(&a_empty[a]);
@@ -240,10 +297,10 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             // warp w may touch lanes 32 * (w % 4) .. + 31 of tensor memory; a thread owns a row of the matrix
             const int quarter = warp & 3, set = warp >> 2, row = quarter * 32 + lane;
             const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
-            const size_t w_row = (size_t)group * p.rows_per_group + (DUAL && set ? p.N : 0) + min(n0 + row, p.N - 1);
-            const uint32_t* scales = p.scales + w_row * p.k_groups + k_first;
-            constexpr int STEP = DUAL ? 1 : SETS;
-            const int first = DUAL ? 0 : set;
+            const Place at(quarter, lane, PAIRED);
+            const uint32_t* scales = p.scales + matrix_row(p, group, n0, at) * p.k_groups + k_first;
+            constexpr int STEP = SETS;
+            const int first = set;
             uint32_t four = first < kgroups ? scales[first] : 0u, next = first + STEP < kgroups ? scales[first + STEP] : 0u;
             bool ok = true;
             for (int i = first; i < kgroups && ok; i += STEP) {
@@ -251,9 +308,9 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                 four = next;
                 if (i + 2 * STEP < kgroups) next = scales[i + 2 * STEP];
                 const int s = i % C::W_STAGES;
-                if (!tc::mbar_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
+                if (!warp_wait(&w_full[s], (i / C::W_STAGES) & 1, abort_flag)) break;
                 uint32_t words[4][4];
-                read_codes(w_tiles + s * C::W_BYTES + (DUAL ? set * CODE_BYTES : 0), row, words);
+                read_codes(w_tiles + s * C::W_BYTES, at.staged, words);
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&w_empty[s]);
 #pragma unroll
@@ -262,36 +319,35 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     if (h >= kblocks) break;
                     uint32_t r[32];
                     half_of(words, p.shifts, by, half, r);
-                    if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    if (!warp_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
-                    tc::tmem_st_x32(tmem_a + lane_part + a * (DUAL ? 64 : 32) + (DUAL ? set * 32 : 0), r);
+                    tc::tmem_st_x32(tmem_a + lane_part + a * 32, r);
                     tc::tmem_st_wait();
                     tc::fence_before_sync();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&a_full[a]);
                 }
             }
-            const int n = n0 + row;
+            const int n = n0 + at.feature;
             const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
             const bool live = n < p.N;
             // epilogue: the sets share the columns
-            const bool done = tc::mbar_wait(acc_bar, 0, abort_flag);
+            const bool done = warp_wait(acc_bar, 0, abort_flag);
             tc::fence_after_sync();
             if (SPLIT) tc::cluster_wait();       // (every thread of the block waits here or below)
             if (done)
 #pragma unroll 1
                 for (int c0 = set * (T / SETS); c0 < (set + 1) * (T / SETS); c0 += 8) {
-                    uint32_t g[8], u[8];
+                    uint32_t g[8];
                     tc::tmem_ld_x8(tmem + lane_part + c0, g);
-                    if (DUAL) tc::tmem_ld_x8(tmem + lane_part + T + c0, u);
                     tc::tmem_ld_wait();
                     if (SPLIT) {                 // to the block that finishes these columns
                         const int width = T / splits, owner = c0 / width;
                         const uint32_t to = tc::map_to_rank(&partial[(rank * width + c0 - owner * width) * BM + row], owner);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) tc::st_cluster_f32(to + j * BM * 4, __uint_as_float(g[j]));
-                    } else if (live)
-                        finish<DUAL>(p, n, bias, row0 + c0, p.rows - row0 - c0, reinterpret_cast<const float*>(g), reinterpret_cast<const float*>(u));
+                    } else
+                        finish_eight<PAIRED>(p, n, live, bias, row0 + c0, p.rows - row0 - c0, reinterpret_cast<const float*>(g));
                 }
             if (SPLIT) {
                 tc::cluster_arrive();
@@ -324,9 +380,9 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
 }
 
-// The same without the gated unit where there are more tiles than SMs: a block an SM that takes tile after tile, with two accumulators, so
+// The same for tiles of 128 rows of which there are more than SMs: a block an SM that takes tile after tile, with two accumulators, so
 // that the epilogue of a tile (eight warps of its own) runs under the products of the next. 4,096 rows of sixteen experts of 2,048 x 2,048 in
-// tiles of 128 rows, float32 results: TBD us, a block a tile 65. What holds it: X, which every block reads for 128 features (L2 gives
+// tiles of 128 rows, float32 results: 52 us, a block a tile 65. What holds it: X, which every block reads for 128 features (L2 gives
 // 12 TB/s), then the instructions of decoding and epilogue.
 template <int T> struct LoopConfig {
     static constexpr int SETS = 4, DEQUANT_WARPS = 16, EPILOGUE_WARPS = 8, THREADS = (DEQUANT_WARPS + EPILOGUE_WARPS + 2) * 32;
@@ -338,7 +394,7 @@ template <int T> struct LoopConfig {
     static_assert(W_STAGES % SETS == 0 && A_STAGES % (2 * SETS) == 0 && 2 * T + A_STAGES * 32 <= 512 && SMEM_BYTES <= 227 * 1024, "tensor or shared memory");
 };
 
-template <int T>
+template <int T, bool PAIRED>
 __global__ void __launch_bounds__(LoopConfig<T>::THREADS, 1)
 gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Mx4Params p) {
     using C = LoopConfig<T>;
@@ -380,7 +436,8 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     dd_launch_dependents();
     dd_grid_wait();              // the tiles' groups and the rows are earlier kernels' results
 
-    const int n_tiles = (p.N + BM - 1) / BM, total = n_tiles * ((p.rows + T - 1) / T);
+    constexpr int FEATURES = features<PAIRED>;
+    const int n_tiles = (p.N + FEATURES - 1) / FEATURES, total = n_tiles * ((p.rows + T - 1) / T);
     // (both halves of the last group, also where K ends in the first: a set then always meets the same stages; zeros by zeros)
     const int kgroups = p.k_groups, kblocks = 2 * kgroups;
     // Every role walks the same tiles; the number of a stage counts on over them. w: groups of 128 k, h: blocks of 64, n: tiles.
@@ -390,13 +447,14 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             int w = 0, h = 0;
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const int group = group_of(tile), n0 = tile % n_tiles * BM, row0 = tile / n_tiles * T;
+                const int group = group_of(tile), n0 = tile % n_tiles * FEATURES, row0 = tile / n_tiles * T, w_row = group * p.rows_per_group + n0;
                 if (group < 0) continue;
                 for (int i = 0; i < kgroups && ok; ++i, ++w) {
                     const int s = w % C::W_STAGES;
                     if (!tc::mbar_wait(&w_empty[s], ((w / C::W_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::mbar_expect_tx(&w_full[s], CODE_BYTES);
-                    tc::tma_load_2d(w_tiles + s * CODE_BYTES, &map_w, i * mx4::GROUP_BYTES, group * p.rows_per_group + n0, &w_full[s]);
+                    tc::tma_load_2d(w_tiles + s * CODE_BYTES, &map_w, i * mx4::GROUP_BYTES, w_row, &w_full[s]);
+                    if (PAIRED) tc::tma_load_2d(w_tiles + s * CODE_BYTES + CODE_BYTES / 2, &map_w, i * mx4::GROUP_BYTES, w_row + p.N, &w_full[s]);
                     for (int half = 2 * i; half < 2 * i + 2; ++half, ++h) {
                         const int x = h % C::X_STAGES;
                         if (!tc::mbar_wait(&x_empty[x], ((h / C::X_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -434,23 +492,24 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             }
         }
     } else if (warp < C::DEQUANT_WARPS) {
-        const int quarter = warp & 3, set = warp >> 2, row = quarter * 32 + lane;
+        const int quarter = warp & 3, set = warp >> 2;
         const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
+        const Place at(quarter, lane, PAIRED);
         int w0 = 0, h0 = 0;                      // of the tile's first group and block
         bool ok = true;
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-            const int group = group_of(tile), n0 = tile % n_tiles * BM;
+            const int group = group_of(tile), n0 = tile % n_tiles * FEATURES;
             if (group < 0) continue;
-            const uint32_t* scales = p.scales + ((size_t)group * p.rows_per_group + min(n0 + row, p.N - 1)) * kgroups;
+            const uint32_t* scales = p.scales + matrix_row(p, group, n0, at) * kgroups;
             const int first = (set - w0 % C::SETS + C::SETS) % C::SETS;
             uint32_t four = first < kgroups ? scales[first] : 0u;
             for (int i = first; i < kgroups && ok; i += C::SETS) {
                 const uint32_t by = four;
                 if (i + C::SETS < kgroups) four = scales[i + C::SETS];
                 const int w = w0 + i, s = w % C::W_STAGES;
-                if (!tc::mbar_wait(&w_full[s], (w / C::W_STAGES) & 1, abort_flag)) { ok = false; break; }
+                if (!warp_wait(&w_full[s], (w / C::W_STAGES) & 1, abort_flag)) { ok = false; break; }
                 uint32_t words[4][4];
-                read_codes(w_tiles + s * CODE_BYTES, row, words);
+                read_codes(w_tiles + s * CODE_BYTES, at.staged, words);
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&w_empty[s]);
 #pragma unroll
@@ -458,7 +517,7 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     const int h = h0 + 2 * i + half, a = h % C::A_STAGES;
                     uint32_t r[32];
                     half_of(words, p.shifts, by, half, r);
-                    if (!tc::mbar_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    if (!warp_wait(&a_empty[a], ((h / C::A_STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     tc::fence_after_sync();
                     tc::tmem_st_x32(tmem_a + lane_part + a * 32, r);
                     tc::tmem_st_wait();
@@ -471,14 +530,15 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             h0 += kblocks;
         }
     } else {
-        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const int quarter = warp & 3;
         const uint32_t lane_part = (uint32_t)(quarter * 32) << 16;
+        const Place at(quarter, lane, PAIRED);
         int number = 0;
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
             if (group_of(tile) < 0) continue;
-            const int n = tile % n_tiles * BM + row, row0 = tile / n_tiles * T;
+            const int n = tile % n_tiles * FEATURES + at.feature, row0 = tile / n_tiles * T;
             const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
-            if (!tc::mbar_wait(&acc_full[number & 1], (number >> 1) & 1, abort_flag)) break;
+            if (!warp_wait(&acc_full[number & 1], (number >> 1) & 1, abort_flag)) break;
             tc::fence_after_sync();
             // two warps a quarter of the lanes, half of the columns each
             const int half = (warp - MMA_WARP - 1) >> 2, count = min(T, p.rows - row0);
@@ -487,10 +547,9 @@ gemm_mx4_loop_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 uint32_t g[16];
                 tc::tmem_ld_x16(tmem + (number & 1) * T + lane_part + c0, g);
                 tc::tmem_ld_wait();
-                if (n < p.N)
 #pragma unroll
-                    for (int j = 0; j < 16; j += 8)
-                        if (c0 + j < count) finish<false>(p, n, bias, row0 + c0 + j, count - c0 - j, reinterpret_cast<const float*>(g + j), nullptr);
+                for (int j = 0; j < 16; j += 8)
+                    if (c0 + j < count) finish_eight<PAIRED>(p, n, n < p.N, bias, row0 + c0 + j, count - c0 - j, reinterpret_cast<const float*>(g + j));
                 __syncwarp();
             }
             tc::fence_before_sync();
@@ -533,15 +592,19 @@ int mx4_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long l
     return 0;
 }
 
-template <int T, bool DUAL, bool SPLIT = false>
-int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, cudaStream_t s, int splits = 1) {
-    using C = Mx4Config<T, DUAL, SPLIT>;
-    cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, DUAL, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
+template <int T, bool PAIRED, bool SPLIT = false>
+int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, int sms, cudaStream_t s, int splits = 1) {
+    using C = Mx4Config<T, SPLIT>;
+    // Three blocks an SM only where two would come in turns (275 blocks: 13.9 us, 18.7 where some SMs took three of them at once; 425: 22.4 and
+    // 19.7): more shared memory keeps the third out.
+    const long long blocks = (long long)dd_ceil_div(p.N, features<PAIRED>) * splits * dd_ceil_div(p.rows, T);
+    const int bytes = C::BLOCKS == 3 && blocks <= 2 * sms ? 80 * 1024 : C::SMEM_BYTES;
+    cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, PAIRED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", bytes, cudaGetErrorString(e));
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(dd_ceil_div(p.N, BM) * splits, dd_ceil_div(p.rows, T));
+    config.gridDim = dim3(dd_ceil_div(p.N, features<PAIRED>) * splits, dd_ceil_div(p.rows, T));
     config.blockDim = dim3(C::THREADS);
-    config.dynamicSmemBytes = C::SMEM_BYTES;
+    config.dynamicSmemBytes = bytes;
     config.stream = s;
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -552,17 +615,17 @@ int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p,
     attrs[1].val.clusterDim.z = 1;
     config.attrs = attrs;
     config.numAttrs = SPLIT ? 2 : 1;
-    e = cudaLaunchKernelEx(&config, gemm_mx4_kernel<T, DUAL, SPLIT>, mw, mx, p);
+    e = cudaLaunchKernelEx(&config, gemm_mx4_kernel<T, PAIRED, SPLIT>, mw, mx, p);
     if (e != cudaSuccess) return dd_fail("dd_gemm_mx4 (clusters of %d): %s", splits, cudaGetErrorString(e));
     return dd_check_launch("dd_gemm_mx4");
 }
-template <int T>
+template <int T, bool PAIRED>
 int launch_loop(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, int sms, cudaStream_t s) {
     using C = LoopConfig<T>;
-    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_loop_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_loop_kernel<T, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
-    const int tiles = dd_ceil_div(p.N, BM) * dd_ceil_div(p.rows, T);
-    dd_launch(gemm_mx4_loop_kernel<T>, dim3(tiles < sms ? tiles : sms), dim3(C::THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);
+    const int tiles = dd_ceil_div(p.N, features<PAIRED>) * dd_ceil_div(p.rows, T);
+    dd_launch(gemm_mx4_loop_kernel<T, PAIRED>, dim3(tiles < sms ? tiles : sms), dim3(C::THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);
     return dd_check_launch("dd_gemm_mx4");
 }
 }  // namespace
@@ -588,7 +651,7 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
     p.ldr = ldr; p.ldo = ldo; p.out_dtype = out_dtype; p.act = act; p.form = form; p.limit = limit; p.alpha = alpha; p.shifts = mx4::SHIFTS;
     const long long row_bytes = (long long)p.k_groups * mx4::GROUP_BYTES;
     CUtensorMap mw, mx;
-    if (int e = mx4_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, (long long)groups * rows_per_group, row_bytes, row_bytes, mx4::GROUP_BYTES, BM,
+    if (int e = mx4_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, (long long)groups * rows_per_group, row_bytes, row_bytes, mx4::GROUP_BYTES, dual ? BM / 2 : BM,
                         CU_TENSOR_MAP_SWIZZLE_64B, "the codes")) return e;
     if (int e = mx4_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, X, rows, K, (long long)ldx * 2, XK, tile, CU_TENSOR_MAP_SWIZZLE_128B, "the rows"))
         return e;
@@ -596,12 +659,12 @@ DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* sc
     // Tiles of 64 rows that would leave most of the GPU idle share K among two, four or eight blocks, as long as each keeps two groups
     // and all fit at once (two an SM).
     int splits = 1;
-    const int tiles = dd_ceil_div(N, BM) * dd_ceil_div(rows, tile);
+    const int tiles = dd_ceil_div(N, dual ? BM / 2 : BM) * dd_ceil_div(rows, tile);
     while (tile == 64 && !dual && !tile_group && splits < 8 && tiles * splits * 2 <= 296 && p.k_groups >= splits * 4) splits *= 2;
-    if (splits > 1) return launch_mx4<64, false, true>(mw, mx, p, s, splits);
-    if (tile == 128 && !dual && tiles > sms) return launch_loop<128>(mw, mx, p, sms, s);      // more tiles than SMs
+    if (splits > 1) return launch_mx4<64, false, true>(mw, mx, p, sms, s, splits);
+    if (tile == 128 && tiles > sms) return dual ? launch_loop<128, true>(mw, mx, p, sms, s) : launch_loop<128, false>(mw, mx, p, sms, s);      // more tiles than SMs
 #define DD_MX4(T) \
-    case T: return dual ? launch_mx4<T, true>(mw, mx, p, s) : launch_mx4<T, false>(mw, mx, p, s);
+    case T: return dual ? launch_mx4<T, true>(mw, mx, p, sms, s) : launch_mx4<T, false>(mw, mx, p, sms, s);
     switch (tile) {
         DD_MX4(16)
         DD_MX4(32)
