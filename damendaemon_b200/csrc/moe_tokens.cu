@@ -111,14 +111,11 @@ template <int KIND> struct Ring {
     int stages, asked = 0, taken = 0;            // stage numbers; their phase follows from how often they wrapped
     uint32_t phase = 0;
     __device__ __forceinline__ Ring(uint64_t* b, uint32_t at, int n) : bars(b), base(at), stages(n) {}
-    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row, int matrix, bool halves) {
+    __device__ __forceinline__ void ask(const CUtensorMap* map, int step, int row, int matrix) {
         uint64_t* bar = &bars[asked];
         uint8_t* slot = reinterpret_cast<uint8_t*>(__cvta_shared_to_generic(base + asked * S::STAGE_BYTES));
         tc::mbar_expect_tx(bar, S::STAGE_BYTES);
-        if (KIND == MX4) {
-            tc::tma_load_4d(slot, map, 0, row, step * S::SUB, matrix, bar);
-            if (!halves) tc::tma_load_4d(slot + S::STAGE_BYTES / 2, map, 0, row + S::HALF, step * S::SUB, matrix, bar);
-        } else tc::tma_load_3d(slot, map, step * S::STEP, row, matrix, bar);
+        tc::tma_load_3d(slot, map, step * (KIND == MX4 ? S::BOX_ROW : S::STEP), row, matrix, bar);
     }
     __device__ __forceinline__ void next_asked() { asked = asked + 1 == stages ? 0 : asked + 1; }
     // the address of the next stage to read; `here`: it has been asked for
@@ -143,14 +140,17 @@ __device__ __forceinline__ void take_column(uint4* b, const __nv_bfloat16* x, in
 #pragma unroll
     for (int i = 0; i < PIECES<KIND>; ++i) b[i] = from[KIND == MX4 ? 4 * i + t : 2 * t + i];
 }
-// The scales of sixteen 4-bit groups of rows g and g + 8: lane (g, t) holds those of groups 4 t .. 4 t + 3, and asks for them a
+// The row of a tile's half that lane (g, t) has: 4-bit rows in another order, so that eight lanes' pieces of a group, under TMA's 128-byte
+// swizzle, meet in no bank (rows r and r + 4 side by side).
+template <int KIND> __device__ __forceinline__ int row_of(int g) { return KIND == MX4 ? g >> 1 | (g & 1) << 2 : g; }
+// The scales of sixteen 4-bit groups of rows g and g + 8 (row_of): lane (g, t) holds those of groups 4 t .. 4 t + 3, and asks for them a
 // stretch of sixteen ahead.
 struct Scales {
     static constexpr int STRETCH = 16;
     uint32_t a[4], b[4];
     __device__ __forceinline__ void load(const uint32_t* rows, size_t row_a, size_t row_b, size_t last, int groups, int from, int to) {
         const int lane = threadIdx.x & 31, first = from + (lane & 3) * 4;
-        const uint32_t *p = rows + min(row_a + (lane >> 2), last) * groups, *q = rows + min(row_b + (lane >> 2), last) * groups;
+        const uint32_t *p = rows + min(row_a + row_of<MX4>(lane >> 2), last) * groups, *q = rows + min(row_b + row_of<MX4>(lane >> 2), last) * groups;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             a[j] = first + j < to ? p[first + j] : 0u;
@@ -171,7 +171,8 @@ template <int KIND, int P, bool F16 = false>
 __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0, uint32_t four1, const uint4 (*b)[PIECES<KIND>], float (*d)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if constexpr (KIND == MX4) {
-        const uint32_t at = slot + sub * 512 + g * 64 + (t ^ (g >> 1 & 3)) * 16;      // [half][group][row][64 bytes]
+        const int row = row_of<KIND>(g);
+        const uint32_t at = slot + row * 128 + ((4 * sub + t) ^ row) * 16;            // [half][row][group]
         const uint4 a0 = few::lds16(at), a1 = few::lds16(at + 1024);
         const uint32_t r0[4] = {a0.x, a0.y, a0.z, a0.w}, r1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
@@ -211,8 +212,9 @@ __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0,
             for (int j = 0; j < 4; ++j) d[p][j] += e[p][j];
     }
 }
+template <int KIND>
 __device__ __forceinline__ void put_tile(Tile& to, const float* d, float by = 1.f) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, g = row_of<KIND>(lane >> 2), t = lane & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i] * by;
 }
@@ -326,7 +328,7 @@ __device__ void partial_logits(const Call& c, const uint8_t* y, int items, Tile*
             if (item != warp) ahead.load(w0, w1, c.l.width, it.from, it.to, c.router_wide);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             few::stream_bf16(w0, w1, x, c.l.width, it.from, it.to, c.router_wide, ahead, d);
-            put_tile(parts[item], d);
+            put_tile<BF16>(parts[item], d);
         }
     }
 }
@@ -615,7 +617,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     if (f_tile < total) f = place_of(f_tile);
     auto fetch = [&] {
         if (f_tile >= total || from >= to) return;
-        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.first, f.matrix, f.unit < 0 || c.l.gated);
+        if (c.w_wide && lane == 0) ring.ask(f.unit < 0 ? &maps.shared_gate_up : &maps.gate_up, f_step, f.first, f.matrix);
         ring.next_asked();
         if (++f_step == to) {
             f_step = from;
@@ -706,10 +708,10 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 }
             }
             if (share > 1) {                      // the first of the sharers adds up
-                put_tile(red[turn][warp], d[0]);
+                put_tile<KIND>(red[turn][warp], d[0]);
                 __syncthreads();
                 if (mine && part == 0) {
-                    const int g = lane >> 2, t = lane & 3;
+                    const int g = row_of<KIND>(lane >> 2), t = lane & 3;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float sum = 0.f;
@@ -720,7 +722,7 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             }
             if (mine && part == 0) {
                 // lane (g, t): features g (and g + 8 of a plain unit) of tokens 2 t and 2 t + 1
-                const int inner = shared ? c.l.shared_inner : c.l.inner, g = lane >> 2;
+                const int inner = shared ? c.l.shared_inner : c.l.inner, g = row_of<KIND>(lane >> 2);
                 const bool gated = shared || c.l.gated;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -794,7 +796,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             f_matrix = matrix_of(unit);
         }
         if (c.inner_wide && lane == 0)
-            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, n0, f_matrix, false);
+            ring.ask(f_shared ? &maps.shared_down : &maps.down, f_at - f_begin, n0, f_matrix);
         ring.next_asked();
         ++f_at;
     };
@@ -884,7 +886,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 // into the tokens that use the expert (the others are not touched: zero times a weight that is not finite is no zero)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    put_tile(columns[warp], d[p], KIND == MX4 ? few::MX4_BACK : 1.f);
+                    put_tile<KIND>(columns[warp], d[p], KIND == MX4 ? few::MX4_BACK : 1.f);
                     __syncwarp();
                     if (lane < 16)
                         for (int i = 0; i < few::COLUMNS && p * few::COLUMNS + i < n * TERMS; ++i)
@@ -927,18 +929,14 @@ int layer_map(CUtensorMap* map, const void* base, long long matrices, long long 
             enc = reinterpret_cast<EncodeTiled>(sym);
     }
     if (!enc) return dd_fail("dd_moe_tokens: cuTensorMapEncodeTiled is not available from this driver");
-    // k, row, matrix; 4 bits: a group's bytes, row, group, matrix, so that a stage holds one group's rows after the other's (and a row's
-    // 64 bytes under the 64-byte swizzle meet in no bank), half the rows of a tile a box
-    constexpr bool FOUR = KIND == MX4;
-    cuuint64_t dims[4] = {(cuuint64_t)(FOUR ? mx4::GROUP_BYTES : K), (cuuint64_t)rows, (cuuint64_t)(FOUR ? row_bytes / mx4::GROUP_BYTES : matrices),
-                          (cuuint64_t)matrices};
-    cuuint64_t strides[3] = {(cuuint64_t)row_bytes, (cuuint64_t)(FOUR ? mx4::GROUP_BYTES : row_bytes * rows), (cuuint64_t)(row_bytes * rows)};
-    cuuint32_t box[4] = {(cuuint32_t)(FOUR ? mx4::GROUP_BYTES : S::STEP), (cuuint32_t)(FOUR ? S::HALF : S::ROWS / box_matrices),
-                         (cuuint32_t)(FOUR ? S::SUB : box_matrices), (cuuint32_t)box_matrices};
-    cuuint32_t elem[4] = {1, 1, 1, 1};
+    // k (of 4-bit rows: bytes), row, matrix
+    cuuint64_t dims[3] = {(cuuint64_t)(KIND == MX4 ? row_bytes : K), (cuuint64_t)rows, (cuuint64_t)matrices};
+    cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(row_bytes * rows)};
+    cuuint32_t box[3] = {(cuuint32_t)(KIND == MX4 ? S::BOX_ROW : S::STEP), (cuuint32_t)(S::ROWS / box_matrices), (cuuint32_t)box_matrices};
+    cuuint32_t elem[3] = {1, 1, 1};
     const CUresult r = enc(map, KIND == F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KIND == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
-                           FOUR ? 4 : 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : FOUR ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                           3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           KIND == F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return dd_fail("dd_moe_tokens: cannot describe %lld matrices of %lld x %d to TMA (driver error %d)", matrices, rows, K, (int)r);
     return 0;
