@@ -76,10 +76,11 @@ quantize_kernel(const T* x, long long ldx, int width, int groups, long long n_gr
         four |= __shfl_xor_sync(mask, four, 8);
         if (lane == 0) scales[first + u] = four;
     }
+    __threadfence();             // (a product may ask for the matrix as soon as this kernel's blocks have ended, before its wait)
 }
 
 // ---------------------------------------------------------------- the values back
-// (Nor may the kernels after this one start before it has ended: it makes the matrix that a product may fetch before its wait.)
+// (Nor may the kernels after this one start before it has ended, as above.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 values_kernel(const uint32_t* codes, const uint32_t* scales, int width, int groups, long long n_groups, T* out, int wide) {
@@ -119,6 +120,7 @@ values_kernel(const uint32_t* codes, const uint32_t* scales, int width, int grou
                 if (k + i < width) to[i] = v[i];
         }
     }
+    __threadfence();
 }
 
 // ---------------------------------------------------------------- the product, few rows

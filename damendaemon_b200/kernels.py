@@ -1553,6 +1553,7 @@ class ExpertLayer:
                  weight_scale=1.0, correction=None, renormalize=False, identity=0, weight_input=False, shared=None, shared_gated=None,
                  shared_gate=False):
         four = isinstance(gate_up, Mx4Matrix)
+        gated, shared_gated = ((tuple(g) + ("clamped_swish",))[:3] if g else None for g in (gated, shared_gated))
         if gate_up.dim() != 3 or down.dim() != 3 or isinstance(down, Mx4Matrix) != four:
             raise KernelError("expert layer: gate_up and down must be stacks of matrices of one kind")
         E, width, inner = gate_up.shape[0], gate_up.shape[2], down.shape[2]

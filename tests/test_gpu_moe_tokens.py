@@ -269,6 +269,13 @@ def test_replayed_beside_eager_calls_and_another_graph(kind):
             assert torch.equal(out, kernels.moe_tokens(part.layer, y, residual))
 
 
+def test_a_form_of_two_numbers_is_the_clamped_one():
+    layer = Layer("bfloat16", 64, 32, 4, 2, unit="clamped_swish")
+    y, residual, _, got = layer.check(3)
+    short = kernels.ExpertLayer(layer.gate_up[0], layer.down[0], 2, gated=layer.form[:2], router=layer.router.to(DEV))
+    assert torch.equal(kernels.moe_tokens(short, y.to(DEV), residual.to(DEV)), got)
+
+
 def test_refusals():
     layer = Layer("bfloat16", 32, 16, 4, 2)
     y = torch.zeros(3, 32, dtype=torch.bfloat16, device=DEV)
