@@ -308,24 +308,25 @@ __device__ __forceinline__ const __nv_bfloat16* router_row(const Call& c, int ti
 template <int KIND>
 __device__ void partial_logits(const Call& c, const uint8_t* y, int items, Tile* parts, few::Ahead& ahead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
-    for (int item = warp; item < items; item += UP_WARPS) {
+    // (float32: four rows of an item a warp)
+    constexpr int PARTS = KIND == F32 ? 16 / few::F32_ROWS : 1;
+    for (int work = warp; work < items * PARTS; work += UP_WARPS) {
+        const int item = work / PARTS;
         const RouterItem it(c, KIND, item);
         if constexpr (KIND == F32) {
-            const int last = c.l.experts + c.l.identity + c.l.shared_gate - 1;
-            for (int r0 = 0; r0 < 16; r0 += few::F32_ROWS) {
-                const float* w[few::F32_ROWS];
-                unsigned long long acc[few::F32_ROWS][MAX_TOKENS] = {};
+            const int last = c.l.experts + c.l.identity + c.l.shared_gate - 1, r0 = work % PARTS * few::F32_ROWS;
+            const float* w[few::F32_ROWS];
+            unsigned long long acc[few::F32_ROWS][MAX_TOKENS] = {};
 #pragma unroll
-                for (int r = 0; r < few::F32_ROWS; ++r)
-                    w[r] = reinterpret_cast<const float*>(c.l.router) + (size_t)min(it.tile * 16 + r0 + r, last) * c.l.router_stride;
-                few::stream_f32<MAX_TOKENS>(w, reinterpret_cast<const float*>(y), c.y_pitch / 4, (1u << c.T) - 1, c.l.width, it.from, it.to, c.router_wide,
-                                            true, acc);
-                put_rows<MAX_TOKENS, false>(parts[item], r0, 0x76543210u, MAX_TOKENS, acc);
-            }
+            for (int r = 0; r < few::F32_ROWS; ++r)
+                w[r] = reinterpret_cast<const float*>(c.l.router) + (size_t)min(it.tile * 16 + r0 + r, last) * c.l.router_stride;
+            few::stream_f32<MAX_TOKENS>(w, reinterpret_cast<const float*>(y), c.y_pitch / 4, (1u << c.T) - 1, c.l.width, it.from, it.to, c.router_wide,
+                                        true, acc);
+            put_rows<MAX_TOKENS, false>(parts[item], r0, 0x76543210u, MAX_TOKENS, acc);
         } else {
             const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(y + min(g, c.T - 1) * c.y_pitch);
             const __nv_bfloat16 *w0 = router_row(c, it.tile, g), *w1 = router_row(c, it.tile, g + 8);
-            if (item != warp) ahead.load(w0, w1, c.l.width, it.from, it.to, c.router_wide);
+            if (work != warp) ahead.load(w0, w1, c.l.width, it.from, it.to, c.router_wide);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             few::stream_bf16(w0, w1, x, c.l.width, it.from, it.to, c.router_wide, ahead, d);
             put_tile<BF16>(parts[item], d);
@@ -516,15 +517,22 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     {
         const int pieces = c.y_pitch / 128 * 8, in = 16 / S::ELEMENT;
         const int by = c.T > 4 ? 2 : c.T > 2 ? 4 : c.T > 1 ? 8 : 16, t = warp / by;          // warps a token
+        constexpr int FLIGHT = 4;                 // pieces that a lane asks for at a time
         if (t < c.T)
 #pragma unroll 1
-            for (int at = (warp % by) * 32 + lane; at < pieces; at += by * 32) {
-                uint4 v;
-                if constexpr (KIND == F32) {
-                    const float4 f = few::load4(reinterpret_cast<const float*>(c.y) + (size_t)t * c.ldy, at * in, width, c.y_wide);
-                    v = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w));
-                } else v = few::load8(reinterpret_cast<const __nv_bfloat16*>(c.y) + (size_t)t * c.ldy, at * in, width, c.y_wide);
-                *reinterpret_cast<uint4*>(y + t * c.y_pitch + at * 16) = v;
+            for (int at = (warp % by) * 32 + lane; at < pieces; at += by * 32 * FLIGHT) {
+                uint4 v[FLIGHT];
+#pragma unroll
+                for (int i = 0; i < FLIGHT; ++i) {
+                    const int piece = at + i * by * 32;          // (behind the row: zeros, and no load)
+                    if constexpr (KIND == F32) {
+                        const float4 f = few::load4(reinterpret_cast<const float*>(c.y) + (size_t)t * c.ldy, piece * in, width, c.y_wide);
+                        v[i] = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w));
+                    } else v[i] = few::load8(reinterpret_cast<const __nv_bfloat16*>(c.y) + (size_t)t * c.ldy, piece * in, width, c.y_wide);
+                }
+#pragma unroll
+                for (int i = 0; i < FLIGHT; ++i)
+                    if (at + i * by * 32 < pieces) *reinterpret_cast<uint4*>(y + t * c.y_pitch + (at + i * by * 32) * 16) = v[i];
             }
     }
     __syncthreads();
@@ -778,7 +786,14 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     auto steps_of = [](int K) { return (K + S::STEP - 1) / S::STEP; };
     const int for_shared = steps_of(c.l.shared_inner), per_unit = steps_of(c.l.inner);
     const int total = for_shared + plan.n_units * per_unit;
-    const int from = (int)((long long)total * warp / W), to = (int)((long long)total * (warp + 1) / W);
+    // a step of the shared unit, which every token uses, takes longer with three times eight columns, whose pieces there are no registers to
+    // ask for ahead: counted in quarters (eight tokens, 2,048 x 2,048 and a shared unit 82.4 -> 71.8 us)
+    const int weight = KIND == F32 || c.T * TERMS <= 2 * few::COLUMNS ? 4 : KIND == BF16 ? 12 : 5;
+    auto border = [&](int w) {
+        const long long at = ((long long)for_shared * weight + (long long)(total - for_shared) * 4) * w / W - (long long)for_shared * weight;
+        return for_shared + (int)(at <= 0 ? -((-at + weight - 1) / weight) : at / 4);
+    };
+    const int from = border(warp), to = border(warp + 1);
     // step -> unit (-1: the shared one), its first step and its end
     auto unit_of = [&](int at) { return at < for_shared ? -1 : (at - for_shared) / per_unit; };
     auto begin_of = [&](int unit) { return unit < 0 ? 0 : for_shared + unit * per_unit; };
@@ -992,7 +1007,8 @@ UpPlan plan_up(const DdExpertLayer& l, int T) {
     // (128 outputs and more leave no room for what eight blocks send)
     const size_t router_bytes = l.router ? (size_t)rows * l.width * S::ELEMENT : 0;
     u.tiles = (rows + 15) / 16;
-    u.shares = u.tiles >= 9 ? 1 : u.tiles >= 5 ? 2 : u.tiles >= 3 ? 4 : u.tiles == 2 ? 8 : 16;
+    u.shares = u.tiles >= 9 ? 1 : u.tiles >= 5 ? 2 : u.tiles >= 3 ? 4 : u.tiles == 2 ? 8 : 16;       // warps of which a tile's columns are
+    if (KIND == F32) u.shares = u.shares > 4 ? u.shares / 4 : 1;                                       // (four by its rows)
     u.cluster = router_bytes <= (64 << 10) ? 1 : router_bytes <= (256 << 10) || u.tiles > 8 ? 4 : 8;
     const size_t scratch = !l.router ? 0 : sizeof(Tile) * u.tiles * u.shares + sizeof(float) * (u.cluster * u.tiles * 16 * MAX_TOKENS +
                                                                               MAX_TOKENS * (2 * outputs + (l.groups > MAX_TOP ? l.groups : MAX_TOP)));
