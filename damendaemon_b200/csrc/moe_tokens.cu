@@ -228,24 +228,31 @@ __device__ __forceinline__ uint32_t list_of(uint32_t users) {
 __device__ __forceinline__ int listed(uint32_t list, int i) { return list >> (4 * i) & 7; }
 
 // float32: a step of four rows by N tokens of a list; row t of the other operand: x + t * ld. Four tokens at a time: registers.
+template <int N> constexpr int AT_ONCE = N < 4 ? N : 4;
+template <int N>
+__device__ __forceinline__ void take_rows(float4* b, const float* x, size_t ld, uint32_t list, int step, int h) {
+#pragma unroll
+    for (int i = 0; i < AT_ONCE<N>; ++i) b[i] = *reinterpret_cast<const float4*>(x + listed(list, h + i) * ld + step * 128 + (threadIdx.x & 31) * 4);
+}
+template <int N>
+__device__ __forceinline__ void fma_rows(uint32_t slot, const float4* b, int h, unsigned long long (*d)[N]) {
+#pragma unroll
+    for (int r = 0; r < few::F32_ROWS; ++r) {
+        const uint4 v = few::lds16(slot + r * 512 + (threadIdx.x & 31) * 16);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE<N>; ++i) {
+            few::fma_pair(d[r][h + i], __uint_as_float(v.x), __uint_as_float(v.y), b[i].x, b[i].y);
+            few::fma_pair(d[r][h + i], __uint_as_float(v.z), __uint_as_float(v.w), b[i].z, b[i].w);
+        }
+    }
+}
 template <int N>
 __device__ __forceinline__ void fma_step(uint32_t slot, const float* x, size_t ld, uint32_t list, int step, unsigned long long (*d)[N]) {
-    constexpr int H = N < 4 ? N : 4;
-    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int h = 0; h < N; h += H) {
-        float4 b[H];
-#pragma unroll
-        for (int i = 0; i < H; ++i) b[i] = *reinterpret_cast<const float4*>(x + listed(list, h + i) * ld + step * 128 + lane * 4);
-#pragma unroll
-        for (int r = 0; r < few::F32_ROWS; ++r) {
-            const uint4 v = few::lds16(slot + r * 512 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-                few::fma_pair(d[r][h + i], __uint_as_float(v.x), __uint_as_float(v.y), b[i].x, b[i].y);
-                few::fma_pair(d[r][h + i], __uint_as_float(v.z), __uint_as_float(v.w), b[i].z, b[i].w);
-            }
-        }
+    for (int h = 0; h < N; h += AT_ONCE<N>) {
+        float4 b[AT_ONCE<N>];
+        take_rows<N>(b, x, ld, list, step, h);
+        fma_rows<N>(slot, b, h, d);
     }
 }
 // The warp's sums of rows r0 .. r0 + 3 and the first n tokens of a list, set or added in `to`.
@@ -844,8 +851,17 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
             by_count(n, [&](auto count) {
                 constexpr int N = decltype(count)::value;
                 unsigned long long d[few::F32_ROWS][N] = {};
+                const float* x = reinterpret_cast<const float*>(c.hidden) + hidden;
+                float4 b[AT_ONCE<N>];             // up to four rows' next step (they come from L2)
+                if constexpr (N <= 4) take_rows<N>(b, x, ld, list, at - begin, 0);
                 for (int s = at; s < end; ++s) {
-                    fma_step<N>(next(s), reinterpret_cast<const float*>(c.hidden) + hidden, ld, list, s - begin, d);
+                    if constexpr (N <= 4) {
+                        float4 now[AT_ONCE<N>];
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE<N>; ++i) now[i] = b[i];
+                        if (s + 1 < end) take_rows<N>(b, x, ld, list, s + 1 - begin, 0);
+                        fma_rows<N>(next(s), now, 0, d);
+                    } else fma_step<N>(next(s), x, ld, list, s - begin, d);
                     __syncwarp();
                     fetch();
                 }
