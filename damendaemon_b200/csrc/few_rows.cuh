@@ -22,13 +22,11 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
 // Eight bfloat16 values of a row from element k on, zeros from element n on; wide: the row is whole 16-byte pieces. (The element by
 // element form is a call: inlined, it would lie between the instructions of every user.)
 static __device__ __noinline__ uint4 load8_slow(const __nv_bfloat16* row, int k, int n) {
-    uint32_t w[4];
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-        w[i] = 0u;
-        if (k + 2 * i < n) w[i] = __bfloat16_as_ushort(row[k + 2 * i]);
-        if (k + 2 * i + 1 < n) w[i] |= (uint32_t)__bfloat16_as_ushort(row[k + 2 * i + 1]) << 16;
-    }
+    uint32_t e[8], w[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = k + i < n ? __bfloat16_as_ushort(row[k + i]) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = e[2 * i] | e[2 * i + 1] << 16;
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int k, int n, bool wide) {

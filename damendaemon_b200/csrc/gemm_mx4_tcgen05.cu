@@ -23,7 +23,8 @@
 // four warps take groups of 128 k in turn. Sets that take turns need stages whose phases they cannot miss, since a wait for the phase
 // after one that has not ended yet passes at once: codes lie in rings whose length the sets divide, so that a stage is always one
 // set's; so does W in its ring of four, and in its ring of three a set that turns to half h (of 64 k) has waited for the products of half h - 6
-// already (its half before that was h - 1 or h - 3, which waited for h - 4 or h - 6), so the phase it asks for is the present one or past. Every wait is
+// already (its half before that was h - 1 or h - 3, which waited for h - 4 or h - 6), so the phase it asks for is the present one or past.
+// Every wait is
 // bounded, and a warp's lanes decide alike.
 #include "common.cuh"
 #include "mx4.cuh"
@@ -108,7 +109,8 @@ __device__ __forceinline__ void read_codes(const uint8_t* tile, int row, uint32_
         words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
     }
 }
-// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales. Scales of 1 .. 128 (all blocks but those of zeros and those whose largest
+// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales. Scales of 1 .. 128 (all blocks but those of
+// zeros and those whose largest
 // element passes 16) need no case of their own.
 __device__ __forceinline__ void half_of(const uint32_t (*words)[4], const mx4::Shifts& shifts, uint32_t four, int half, uint32_t* r) {
     const bool easy = ((four - 0x01010101u) & 0x80808080u) == 0;
@@ -171,7 +173,8 @@ __device__ __forceinline__ void finish(const Mx4Params& p, int n, float bias, in
     else columns(Act<DD_ACT_TANH>{}, As<float>{});
 }
 
-// The features of a block, and where a thread finds its own: lane `quarter * 32 + lane` of the accumulator is that feature's row, or, PAIRED, lanes
+// The features of a block, and where a thread finds its own: lane `quarter * 32 + lane` of the accumulator is that feature's row, or,
+// PAIRED, lanes
 // 0 .. 15 of a quarter are the gate rows of sixteen features and 16 .. 31 their up rows (in the stage: 64 gate rows, then 64 up rows).
 template <bool PAIRED> constexpr int features = PAIRED ? BM / 2 : BM;
 struct Place {
@@ -631,7 +634,8 @@ int launch_loop(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p
 }  // namespace
 
 // X [rows, K] bf16 (row stride ldx) in tiles of `tile` rows (16, 32, 64, 128); codes, scales: `groups` 4-bit matrices of rows_per_group
-// rows of K; tile_group: device array [rows / tile] (a negative group's tile is skipped, so is one out of range, with error bit 1), or null: one matrix for
+// rows of K; tile_group: device array [rows / tile] (a negative group's tile is skipped, so is one out of range, with error bit 1), or
+// null: one matrix for
 // all rows, of which the last tile may hold fewer. dual == 0: rows_per_group == N, act(row_scale * sum + bias) + residual; dual != 0:
 // rows_per_group == 2 N, the gated unit. out: [rows, N] bf16 or f32, row stride ldo.
 DD_API int dd_gemm_mx4(const void* X, int ldx, const void* codes, const void* scales, int groups, int rows_per_group, const int* tile_group,

@@ -231,6 +231,18 @@ void launch_rows(const RowsParams& p, int kw, cudaStream_t s) {
     else dd_launch(gemm_mx4_rows_kernel<NT, 8>, grid, dim3(THREADS), 0, s, p);
 }
 
+// out[M, width] = the rows of X and zeros behind them, a thread eight neighbours: rows that are no whole 16-byte pieces, as TMA wants them.
+__global__ void __launch_bounds__(THREADS)
+pad_rows_kernel(const __nv_bfloat16* X, long long ldx, int K, int width, long long pieces, uint4* out) {
+    dd_launch_dependents();
+    dd_grid_wait();
+    const int per_row = width / 8;
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < pieces; i += (long long)gridDim.x * THREADS) {
+        const long long row = i / per_row;
+        out[i] = few::load8(X + row * ldx, (int)(i - row * per_row) * 8, K, false);
+    }
+}
+
 bool rows_of_16_bytes(const void* base, long long ld, int width, int element) {
     return !((uintptr_t)base & 15) && ld * element % 16 == 0 && width % 8 == 0;
 }
@@ -275,6 +287,16 @@ DD_API int dd_mx4_values(const void* codes, const void* scales, long long rows, 
     else
         return dd_fail("dd_mx4_values: unknown dtype %d", dtype);
     return dd_check_launch("dd_mx4_values");
+}
+
+// out [rows, width] bfloat16: the rows of X [rows, K] (row stride ldx), then zeros; width: K rounded up to a multiple of 8.
+DD_API int dd_mx4_pad_rows(const void* X, long long ldx, long long rows, int K, int width, void* out, void* stream) {
+    if (rows <= 0 || K <= 0) return 0;
+    if (width % 8 || width < K || ((uintptr_t)out & 15)) return dd_fail("dd_mx4_pad_rows: rows of %d elements as rows of %d", K, width);
+    const long long pieces = rows * (width / 8), blocks = (pieces + THREADS - 1) / THREADS;
+    dd_launch(pad_rows_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(THREADS), 0, (cudaStream_t)stream, (const __nv_bfloat16*)X, ldx, K,
+              width, pieces, (uint4*)out);
+    return dd_check_launch("dd_mx4_pad_rows");
 }
 
 // out[M, N] = act(X . W^T + bias) (+ residual), X bfloat16 [M, ldx], W the 4-bit matrix [N, K].

@@ -108,8 +108,8 @@ __device__ __forceinline__ uint32_t dd_best_key(const uint32_t* key, int* at) {
     *at = (int)__reduce_min_sync(0xffffffffu, first);
     return best;
 }
-// dd_choose_experts for at most 32 N experts: the same choice and the same weights, with the scores in registers (see dd_choose_experts for what it measures
-// instead of 3.2). worth: max(groups, top) numbers of scratch.
+// dd_choose_experts for at most 32 N experts: the same choice and the same weights, with the scores in registers (two of sixteen in
+// 0.7 us). worth: max(groups, top) numbers of scratch.
 template <int N>
 __device__ __forceinline__ void dd_choose_few(float* score, float* value, float* worth, int n_experts, int top, int groups, int keep, float weight_scale,
                                               int softmax, const float* correction, int renormalize, int* chosen, float* pair_weight) {

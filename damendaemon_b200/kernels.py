@@ -109,6 +109,7 @@ _SIGNATURES = {
         "dd_moe_tokens": [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
         "dd_mx4_quantize": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_int, _c_void],
         "dd_mx4_values": [_c_void, _c_void, ctypes.c_longlong, _c_int, _c_void, _c_int, _c_void],
+        "dd_mx4_pad_rows": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_int, _c_void, _c_void],
         "dd_gemm_mx4_rows": [_c_void, _c_int] + [_c_void] * 4 + [_c_int, _c_void] + [_c_int] * 6 + [_c_void],
         "dd_sample": [_c_void, _c_int, _c_int, _c_int] + [_c_void] * 6,
         "dd_adjust_logits": [_c_void, _c_int, _c_int] + [_c_void] * 8 + [_c_int, _c_void],
@@ -1622,7 +1623,9 @@ def moe_tokens(layer, y, residual=None, ids=None, out=None):
     """A whole expert layer for one to layer.most_tokens tokens (eight, fewer where rows are very wide) in two kernels: routing, the
     chosen units, the shared unit, the weighted sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the
     layer's dtype; ids int32 [T] for a layer by table; out float32 (residual itself may be given). Sums are float32; a hidden row meets
-    the down matrix as float32, in bfloat16 layers as the sum of three bfloat16 numbers (24 bits). An expert or token id out of range sets error bit 1 and is left out."""
+    the down matrix as float32, in bfloat16 layers as the sum of three bfloat16 numbers (24 bits). 4-bit layers: y's elements are kept
+    exactly down to 2^-31 of their row's largest and to 2^-39 of it below that, and hidden values must be smaller than
+    2^63 in size. An expert or token id out of range sets error bit 1 and is left out."""
     T = y.shape[0]
     if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > layer.most_tokens:
         raise KernelError(f"moe_tokens: rows {tuple(y.shape)} {y.dtype} do not fit a layer of width {layer.width} {layer.dtype} "
@@ -1739,24 +1742,33 @@ def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, ou
     of_bias, of_residual = bias, residual
     bias, residual_stride = _ptr(bias, "bias", torch.float32), 0 if residual is None else residual.stride(0)
     residual = _ptr(residual, "residual", torch.float32)
-    if not _mx4_rows(M, N, K) and K % 8 == 0 and a.stride(0) % 8 == 0 and pointer % 16 == 0:
-        if M > MX4_FUSED_ROWS:
-            return gemm_tcgen05(a, mx4_values(w), of_bias, of_residual, activation, out_dtype, out)
-        _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), 1, N, None, bias, residual,
-              residual_stride, None, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, 64, 0, 0.0, 0.0, 0,
-              ACTIVATIONS[activation], kind, sm_count(a.device), _ptr(error_flag(a.device)), _stream())
-    else:
+    as_they_are = M <= MX4_UNPADDED_ROWS or 2 * M * N * K <= MX4_SMALL
+    if not as_they_are and (K % 8 or a.stride(0) % 8 or pointer % 16):
+        # rows of whole 16-byte pieces, zeros behind K (so has the matrix, up to a whole group)
+        rows, K = a, -(-K // 8) * 8
+        a = torch.empty((M, K), dtype=torch.bfloat16, device=rows.device)
+        _call(library("core"), "dd_mx4_pad_rows", pointer, rows.stride(0), M, rows.shape[1], K, a.data_ptr(), _stream())
+        w, pointer = Mx4Matrix(w.codes, w.scales, K), a.data_ptr()
+    if as_they_are or _mx4_rows(M, N, K):
         _call(library("core"), "dd_gemm_mx4_rows", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), bias, residual,
               residual_stride, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, ACTIVATIONS[activation], kind, _stream())
+        return out
+    if M > MX4_FUSED_ROWS:
+        return gemm_tcgen05(a, mx4_values(w), of_bias, of_residual, activation, out_dtype, out)
+    _call(library("tensor"), "dd_gemm_mx4", pointer, a.stride(0), _ptr(w.codes, "w"), w.scales.data_ptr(), 1, N, None, bias, residual,
+          residual_stride, None, _ptr(out, "out", out_dtype), out.stride(0), M, N, K, 64, 0, 0.0, 0.0, 0,
+          ACTIVATIONS[activation], kind, sm_count(a.device), _ptr(error_flag(a.device)), _stream())
     return out
 
 
-MX4_FEW_ROWS, MX4_SMALL, MX4_FUSED_ROWS = 32, 1 << 26, 256
+# (rows that are no whole 16-byte pieces: 16 x 1,601 -> 6,400 15.3 us as they are and 7.8 copied first, 32 43.8 and 14.9, 8 8.7 and 5.8; 32 x 999
+# -> 1,030 13.3 and 6.3; the copy costs the host 9)
+MX4_FEW_ROWS, MX4_SMALL, MX4_FUSED_ROWS, MX4_UNPADDED_ROWS = 32, 1 << 26, 256, 16
 
 
 def _mx4_rows(M, N, K):
-    """Whether a product with a 4-bit matrix streams it through mma.sync (any rows and strides): up to 32 rows, and small
-    products (61 x 1,030 x 1,000 5.0 us, 7.5 on tcgen05; 33 x 1,600 x 6,400 16.1 and 11.5)."""
+    """Whether a product with a 4-bit matrix streams it through mma.sync: up to 32 rows, and small products (61 x 1,030 x 1,000
+    5.0 us, 7.5 on tcgen05; 33 x 1,600 x 6,400 16.1 and 11.5)."""
     return M <= MX4_FEW_ROWS or M * N * K <= MX4_SMALL
 
 

@@ -167,6 +167,20 @@ def test_gemm_mx4_wide_scales(path, M):
     close(kernels.gemm_mx4(a.to(DEV), q, out_dtype=torch.float32), a.double() @ values.t(), product_bound(a, values, 1))
 
 
+@pytest.mark.parametrize("M,N,K", [(17, 96, 999), (40, 130, 1601), (200, 64, 97), (270, 140, 805), (300, 33, 7)])
+def test_gemm_mx4_rows_of_no_whole_pieces(path, M, N, K):
+    """More rows than go through mma.sync as they are: widths that are no multiple of 8, a stride or a start between 16-byte boundaries."""
+    w = kernels.mx4_quantize(randn(K, N, K, scale=K ** -0.5).to(DEV))
+    values = kernels.mx4_values(w, torch.float32).double().cpu()
+    store, bias, residual = randn(M, M, K + 11, dtype=torch.bfloat16), randn(1, N), randn(2, M, N)
+    for a in (store[:, :K].contiguous(), store[:, 3:K + 3], store[:, 8:K + 8]):
+        want, bound = a.double() @ values.t(), product_bound(a, values)
+        close(kernels.gemm_mx4(a.to(DEV) if a.is_contiguous() else store.to(DEV)[:, a.storage_offset():a.storage_offset() + K], w,
+                               out_dtype=torch.float32), want, bound)
+        got = kernels.gemm_mx4(a.to(DEV), w, bias.to(DEV), residual.to(DEV), None, torch.float32)
+        close(got, want + bias.double() + residual.double(), bound + 2.0 ** -22 * (want.abs() + bias.abs() + residual.abs() + 1))
+
+
 @pytest.mark.parametrize("M", [2, 70])
 def test_gemm_mx4_not_finite(path, M):
     w, a = randn(1, 40, 160), randn(2, M, 160, dtype=torch.bfloat16)
