@@ -55,6 +55,7 @@ struct GemmParams {
     int vec;                     // out, residual and bias allow 16-byte accesses at every row start (tiles of 128 tokens)
     const uint8_t* prefetch;        // null, or memory a later kernel will stream (the next weight matrix):
     unsigned long long prefetch_bytes;   // every block asks L2 to fetch its share while this kernel runs
+    int fresh_weights;           // W is the result of a kernel before this one: no tile of it is asked for before dd_grid_wait
 };
 
 
@@ -362,8 +363,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             tc::prefetch_tensormap(&map_b);
             uint32_t it = 0;                               // k-blocks issued so far, across items
             bool ok = true;
-            // Weights never change, so the weight tiles of the first stages are requested before the
-            // kernel that produces the activations has finished; the activation tiles follow the wait.
+            // Weights do not change while a model runs, so the weight tiles of the first stages are requested before the
+            // kernel that produces the activations has finished; the activation tiles follow the wait. (A matrix that a kernel
+            // has just made is waited for: fresh_weights.)
+            if (p.fresh_weights) dd_grid_wait();
             int ahead = 0;
             if (blockIdx.x < n_items) {
                 DD_ITEM_COORDS(blockIdx.x)
@@ -665,7 +668,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
             tc::prefetch_tensormap(&map_w);
             tc::prefetch_tensormap(&map_x);
             // Weights do not depend on the kernel before this one: the weight halves of the first tile's first stages
-            // are on their way before the wait; the activations follow after it.
+            // are on their way before the wait (unless that kernel made them); the activations follow after it.
+            if (p.fresh_weights) dd_grid_wait();
             int ahead = 0;
             if (pair < n_items) {
                 const int b_first = (pair / tiles_a) * BN;
@@ -887,7 +891,8 @@ gemm_tcgen05_cluster_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         if (tc::elect_one()) {
             tc::prefetch_tensormap(&map_w);
             tc::prefetch_tensormap(&map_x);
-            // weights first: they do not depend on the kernel before this one
+            // weights first: they do not depend on the kernel before this one (unless it made them)
+            if (p.fresh_weights) dd_grid_wait();
             const int ahead = min(n_kblocks, C::STAGES);
             for (int i = 0; i < ahead; ++i) {
                 tc::mbar_expect_tx(&full_bar[i], C::STAGE_BYTES);
@@ -1240,11 +1245,12 @@ DD_API int dd_gemm_tcgen05_plan(int M, int N, int K, int sm_count, int* token_ti
 // (token_tile <= 64); cluster = 3: the same with rings of 10 stages and one block per SM (token_tile 16); cluster = 2: two SMs per tile of 256 tokens x token_tile features (tcgen05
 // cta_group::2), token_tile 128/192/256; cluster = 0 with splits > 1 (token_tile <= 64): workspace f32
 // [splits*M*N] and counters int32 [tiles], zero before the first launch. prefetch/prefetch_bytes: null/0, or memory that a later kernel streams once (the next
-// weight matrix of a decode step): this kernel's blocks ask L2 to fetch it while they run.
+// weight matrix of a decode step): this kernel's blocks ask L2 to fetch it while they run. fresh_weights: W was written by a kernel
+// of this stream that may still be running when this one starts; its tiles are then asked for behind the wait.
 DD_API int dd_gemm_tcgen05(const void* X, int ldx, const void* W, int ldw, const float* bias, const float* residual,
                            int ldr, void* out, int ldo, int M, int N, int K, int act, int out_dtype, int splits,
                            int token_tile, int cluster, float* workspace, int* counters, int n_counters,
-                           const void* prefetch, long long prefetch_bytes, int* error_flag, void* stream) {
+                           const void* prefetch, long long prefetch_bytes, int fresh_weights, int* error_flag, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || K % 8 || ldx % 8 || ldw % 8)
         return dd_fail("dd_gemm_tcgen05: K=%d and the row strides (%d, %d) must be multiples of 8 (TMA needs 16-byte rows)", K, ldx, ldw);
@@ -1262,6 +1268,7 @@ DD_API int dd_gemm_tcgen05(const void* X, int ldx, const void* W, int ldw, const
     p.error_flag = error_flag; p.M = M; p.N = N; p.K = K; p.ldr = ldr; p.ldo = ldo; p.act = act; p.out_dtype = out_dtype;
     p.prefetch = (const uint8_t*)prefetch;
     p.prefetch_bytes = (prefetch && prefetch_bytes > 0 && !((uintptr_t)prefetch & 15)) ? (unsigned long long)prefetch_bytes : 0;
+    p.fresh_weights = fresh_weights;
     p.splits = splits; p.kblocks_per_split = dd_ceil_div(kblocks, splits);
     p.splits = dd_ceil_div(kblocks, p.kblocks_per_split);     // no empty split
     if (p.splits == 1 && (cluster == 1 || cluster == 3)) cluster = 0;

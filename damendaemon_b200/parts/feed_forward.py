@@ -23,7 +23,7 @@ def _held(runtime, w):
     """A feed-forward's matrix, or stack of matrices, as the runtime wants it held."""
     if runtime.feed_forward != "mx4" or isinstance(w, kernels.Mx4Matrix):
         return w
-    return kernels.mx4_quantize(w)
+    return kernels.mx4_quantize(w).settle()
 
 
 def _take(runtime, weights, name):
