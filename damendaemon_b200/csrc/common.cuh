@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 
 #define DD_API extern "C" __attribute__((visibility("default")))
 
@@ -137,4 +138,18 @@ static inline cudaError_t dd_launch(void (*kernel)(KArgs...), dim3 grid, dim3 bl
     config.attrs = attribute;
     config.numAttrs = dd_pdl_enabled ? 1 : 0;
     return cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...);
+}
+
+// Lets a kernel ask for up to `bytes` of dynamic shared memory: told to the driver once a device, always the same number, so that
+// calls of other threads cannot lower it between here and the launch (two threads that are first tell the same).
+template <auto KERNEL>
+static cudaError_t dd_allow_shared(int bytes) {
+    constexpr int DEVICES = 64;
+    static std::atomic<bool> told[DEVICES];
+    int d = -1;
+    const bool kept = cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < DEVICES;
+    if (kept && told[d].load(std::memory_order_acquire)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (kept && e == cudaSuccess) told[d].store(true, std::memory_order_release);
+    return e;
 }

@@ -601,9 +601,10 @@ int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p,
     // Three blocks an SM only where two would come in turns (275 blocks: 13.9 us, 18.7 where some SMs took three of them at once; 425: 22.4 and
     // 19.7): more shared memory keeps the third out.
     const long long blocks = (long long)dd_ceil_div(p.N, features<PAIRED>) * splits * dd_ceil_div(p.rows, T);
-    const int bytes = C::BLOCKS == 3 && blocks <= 2 * sms ? 80 * 1024 : C::SMEM_BYTES;
-    cudaError_t e = cudaFuncSetAttribute(gemm_mx4_kernel<T, PAIRED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", bytes, cudaGetErrorString(e));
+    constexpr int TWO_FIT = 80 * 1024, MOST = C::BLOCKS == 3 && TWO_FIT > C::SMEM_BYTES ? TWO_FIT : C::SMEM_BYTES;
+    const int bytes = C::BLOCKS == 3 && blocks <= 2 * sms ? TWO_FIT : C::SMEM_BYTES;
+    cudaError_t e = dd_allow_shared<gemm_mx4_kernel<T, PAIRED, SPLIT>>(MOST);
+    if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", MOST, cudaGetErrorString(e));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(dd_ceil_div(p.N, features<PAIRED>) * splits, dd_ceil_div(p.rows, T));
     config.blockDim = dim3(C::THREADS);
@@ -625,7 +626,7 @@ int launch_mx4(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p,
 template <int T, bool PAIRED>
 int launch_loop(const CUtensorMap& mw, const CUtensorMap& mx, const Mx4Params& p, int sms, cudaStream_t s) {
     using C = LoopConfig<T>;
-    const cudaError_t e = cudaFuncSetAttribute(gemm_mx4_loop_kernel<T, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    const cudaError_t e = dd_allow_shared<gemm_mx4_loop_kernel<T, PAIRED>>(C::SMEM_BYTES);
     if (e != cudaSuccess) return dd_fail("dd_gemm_mx4: shared memory of %d bytes refused: %s", C::SMEM_BYTES, cudaGetErrorString(e));
     const int tiles = dd_ceil_div(p.N, features<PAIRED>) * dd_ceil_div(p.rows, T);
     dd_launch(gemm_mx4_loop_kernel<T, PAIRED>, dim3(tiles < sms ? tiles : sms), dim3(C::THREADS), (size_t)C::SMEM_BYTES, s, mw, mx, p);

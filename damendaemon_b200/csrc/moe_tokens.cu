@@ -991,6 +991,8 @@ int layer_maps(Maps* m, const DdExpertLayer& l) {
     return layer_map<KIND>(&m->shared_down, l.shared_down, 1, l.width, l.shared_inner, 1);
 }
 
+// Dynamic shared memory of up_kernel, at most: less the static part.
+constexpr size_t MOST_SHARED = 227 * 1024 - 32 * 1024;
 template <int KIND>
 int launch_up(const Call& c, const Maps& m, int blocks, size_t smem, cudaStream_t s) {
     cudaLaunchConfig_t config = {};
@@ -1007,7 +1009,7 @@ int launch_up(const Call& c, const Maps& m, int blocks, size_t smem, cudaStream_
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attrs;
     config.numAttrs = dd_pdl_enabled ? 2 : 1;
-    cudaError_t e = cudaFuncSetAttribute(up_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = dd_allow_shared<up_kernel<KIND>>((int)MOST_SHARED);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, up_kernel<KIND>, c, m);
     if (e != cudaSuccess) return dd_fail("dd_moe_tokens (clusters of %d, %d bytes of shared memory): %s", c.cluster, (int)smem, cudaGetErrorString(e));
     return dd_check_launch("dd_moe_tokens");
@@ -1015,7 +1017,7 @@ int launch_up(const Call& c, const Maps& m, int blocks, size_t smem, cudaStream_
 template <int KIND, int W>
 int launch_down(const Call& c, const Maps& m, int tiles, cudaStream_t s) {
     constexpr int BYTES = W * Stream<KIND>::MOST_STAGES * Stream<KIND>::STAGE_BYTES + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(down_kernel<KIND, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    const cudaError_t e = dd_allow_shared<down_kernel<KIND, W>>(BYTES);
     if (e != cudaSuccess) return dd_fail("dd_moe_tokens: shared memory of %d bytes refused: %s", BYTES, cudaGetErrorString(e));
     dd_launch(down_kernel<KIND, W>, dim3(tiles), dim3(W * 32), (size_t)BYTES, s, c, m);
     return dd_check_launch("dd_moe_tokens");
@@ -1023,7 +1025,6 @@ int launch_down(const Call& c, const Maps& m, int tiles, cudaStream_t s) {
 
 // How up_kernel shares its routing and its shared memory out.
 struct UpPlan { int tiles, shares, cluster, y_pitch; size_t fixed, stage; };
-constexpr size_t MOST_SHARED = 227 * 1024 - 32 * 1024;       // less the static part
 template <int KIND>
 UpPlan plan_up(const DdExpertLayer& l, int T) {
     using S = Stream<KIND>;

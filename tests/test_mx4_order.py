@@ -67,3 +67,12 @@ def test_a_matrix_is_read_early_only_where_it_is_settled(launches, monkeypatch, 
         args = launches.calls[-1][1]
         assert launches.calls[-1][0] == "dd_gemm_mx4_rows" and len(args) == len(kernels._SIGNATURES["core"]["dd_gemm_mx4_rows"])
         assert args[-2] == int(settled)
+
+
+def test_limits_of_shared_memory_are_told_once():
+    """A launcher that told the driver another limit for every call's size could lower the one that another thread's call has
+    just raised. dd_allow_shared tells one constant a kernel."""
+    from damendaemon_b200.csrc import build
+    for name in ("moe_tokens.cu", "gemm_mx4_tcgen05.cu"):
+        source = (build.HERE / name).read_text()
+        assert "cudaFuncSetAttribute" not in source and "dd_allow_shared<" in source
