@@ -153,7 +153,7 @@ __device__ __forceinline__ void finish(const Mx4Params& p, int n, float bias, in
         for (int j = 0; j < MOST; ++j) {
             if (j >= count) break;
             float v = g[j];
-            if (PAIRED) v = dd_gated_value<true>(v, u[j], p.form, p.limit, p.alpha);
+            if (PAIRED) v = dd_gated_value<DdType<Out>::id == DD_BF16>(v, u[j], p.form, p.limit, p.alpha);
             else {
                 if (p.row_scale) v *= p.row_scale[r + j];
                 v += bias;
