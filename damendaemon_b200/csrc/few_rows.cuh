@@ -38,20 +38,10 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int k, int n, b
 // Asks L2 for the line of an address, whatever wrote it: no value is taken, so it may stand before dd_grid_wait where a load may not.
 __device__ __forceinline__ void ask_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at) : "memory"); }
 
-// X times 2^64: the other operand's elements are times 2^-126, and the products must stay clear of float32's smallest numbers.
-// |x| has to be below 2^63 (beyond it the result is not finite); sums below 2^-64 may be lost.
-constexpr float MX4_BACK = 4.611686018427387904e18f;         // 2^62: what is left of both factors
-__device__ __forceinline__ uint32_t lift(uint32_t pair) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(0x5F805F80u));
-    return r;
-}
-}  // namespace few
-
-namespace few {
 // ---------------------------------------------------------------- a warp's share of a product, 16 rows of W by eight rows of X
 // W bfloat16: steps of 32 k, two instructions each, AHEAD steps requested at a time. w0, w1: rows g and g + 8 of W; x: row g of X
-// (whole 16-byte pieces). `have` holds what Ahead::load fetched of the first steps, before X was there. (For matrices of a few rows, which come from L2; the large ones go through rings.)
+// (whole 16-byte pieces). `have` holds what Ahead::load fetched of the first steps, before X was there. (For matrices of a few rows, which
+// come from L2; the large ones go through rings.)
 struct Ahead {
     static constexpr int STEPS = 6;
     uint4 a0[STEPS], a1[STEPS];
@@ -93,11 +83,10 @@ __device__ __forceinline__ void stream_bf16(const __nv_bfloat16* w0, const __nv_
 }
 
 // A block of 32 elements of rows g and g + 8 of a 4-bit W (a lane's word of each) by its eight elements of X, into an accumulator
-// of its own; add_block adds that, times the block's scales, to the float32 sums: the elements need no multiplication. The sums are
-// times 1 / MX4_BACK.
+// of its own; add_block adds that, times the block's scales, to the float32 sums: the elements need no scale of their own.
 __device__ __forceinline__ void block_product(const uint32_t* v0, const uint32_t* v1, uint4 x, float* d) {
-    mma(d, v0[0], v1[0], v0[1], v1[1], lift(x.x), lift(x.y));
-    mma(d, v0[2], v1[2], v0[3], v1[3], lift(x.z), lift(x.w));
+    mma(d, v0[0], v1[0], v0[1], v1[1], x.x, x.y);
+    mma(d, v0[2], v1[2], v0[3], v1[3], x.z, x.w);
 }
 __device__ __forceinline__ void add_block(float by0, float by1, const float* d, float* acc) {
     acc[0] = fmaf(by0, d[0], acc[0]);

@@ -87,7 +87,7 @@ __device__ __forceinline__ float gelu_new_fast(float u) {
 }
 // The factor of a block's pairs (mx4::pairs): 2^126 * 2^(s - 127), twice in a register; above 2^127 what is missing comes later.
 __device__ __forceinline__ uint32_t pair_factor(uint32_t s) {
-    const uint32_t bits = s == 0 ? 0u : s == 255 ? 0x7fc0u : (min(s, 128u) + 126u) << 7;
+    const uint32_t bits = s == 255 ? 0x7fc0u : (min(s, 128u) + 126u) << 7;
     return bits | (bits << 16);
 }
 
@@ -109,11 +109,10 @@ __device__ __forceinline__ void read_codes(const uint8_t* tile, int row, uint32_
         words[t][0] = v.x; words[t][1] = v.y; words[t][2] = v.z; words[t][3] = v.w;
     }
 }
-// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales. Scales of 1 .. 128 (all blocks but those of
-// zeros and those whose largest
-// element passes 16) need no case of their own.
+// Half of them (64 k, two blocks) as bfloat16 pairs in the order of k, times their scales. Scales of 0 .. 127 (all blocks but those whose
+// largest element passes 8) need no case of their own.
 __device__ __forceinline__ void half_of(const uint32_t (*words)[4], const mx4::Shifts& shifts, uint32_t four, int half, uint32_t* r) {
-    const bool easy = ((four - 0x01010101u) & 0x80808080u) == 0;
+    const bool easy = (four & 0x80808080u) == 0;
     uint32_t scale[2], factor[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {

@@ -181,7 +181,7 @@ __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0,
         for (int i = 0; i < 4; ++i) {
             uint32_t v0[4], v1[4];
             if (F16) { mx4::pairs_f16(r0[i], v0); mx4::pairs_f16(r1[i], v1); }
-            else { mx4::pairs(r0[i], v0); mx4::pairs(r1[i], v1); }
+            else { mx4::whole_pairs(r0[i], v0); mx4::whole_pairs(r1[i], v1); }
             const float by0 = mx4::scale(four0, i), by1 = mx4::scale(four1, i);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -215,10 +215,10 @@ __device__ __forceinline__ void mma_step(uint32_t slot, int sub, uint32_t four0,
     }
 }
 template <int KIND>
-__device__ __forceinline__ void put_tile(Tile& to, const float* d, float by = 1.f) {
+__device__ __forceinline__ void put_tile(Tile& to, const float* d) {
     const int lane = threadIdx.x & 31, g = row_of<KIND>(lane >> 2), t = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i] * by;
+    for (int i = 0; i < 4; ++i) to.sum[g + 8 * (i >> 1)][2 * t + (i & 1)] = d[i];
 }
 
 // Up to eight token numbers, ascending, four bits each.
@@ -927,7 +927,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 // into the tokens that use the expert (the others are not touched: zero times a weight that is not finite is no zero)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    put_tile<KIND>(columns[warp], d[p], KIND == MX4 ? few::MX4_BACK : 1.f);
+                    put_tile<KIND>(columns[warp], d[p]);
                     __syncwarp();
                     if (lane < 16)
                         for (int i = 0; i < few::COLUMNS && p * few::COLUMNS + i < n * TERMS; ++i)

@@ -202,19 +202,14 @@ gemm_mx4_rows_kernel(const RowsParams p) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 uint32_t v0[4], v1[4];
-                mx4::pairs(a0[b], v0);
-                mx4::pairs(a1[b], v1);
+                mx4::whole_pairs(a0[b], v0);
+                mx4::whole_pairs(a1[b], v1);
                 const float by0 = mx4::scale(f0[u], b), by1 = mx4::scale(f1[u], b);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint4 y = xv[j][b];
                     float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    few::mma(d, v0[0], v1[0], v0[1], v1[1], few::lift(y.x), few::lift(y.y));
-                    few::mma(d, v0[2], v1[2], v0[3], v1[3], few::lift(y.z), few::lift(y.w));
-                    acc[j][0] = fmaf(by0, d[0], acc[j][0]);
-                    acc[j][1] = fmaf(by0, d[1], acc[j][1]);
-                    acc[j][2] = fmaf(by1, d[2], acc[j][2]);
-                    acc[j][3] = fmaf(by1, d[3], acc[j][3]);
+                    few::block_product(v0, v1, xv[j][b], d);
+                    few::add_block(by0, by1, d, acc[j]);
                 }
             }
         }
@@ -230,7 +225,7 @@ gemm_mx4_rows_kernel(const RowsParams p) {
         float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < KW; ++s) sum += red[(row >> 4) * KW + s][row & 15][i / (RW * 16)];
-        float v = dd_activation(sum * few::MX4_BACK + (p.bias ? p.bias[n] : 0.f), p.act);
+        float v = dd_activation(sum + (p.bias ? p.bias[n] : 0.f), p.act);
         if (p.residual) v += p.residual[(size_t)m * p.ldr + n];
         if (p.out_dtype == DD_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(v);
         else reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + n] = v;
