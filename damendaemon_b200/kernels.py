@@ -104,7 +104,7 @@ _SIGNATURES = {
         "dd_post_norm": [_c_void, _c_void, _c_void, _c_float, _c_float, _c_void, _c_int, _c_void, _c_float, _c_float, _c_void, _c_int,
                          _c_int, _c_int, _c_void],
         "dd_round_rows": [_c_void, _c_void, ctypes.c_longlong, _c_void],
-        "dd_moe_tokens_maps": [_c_void, _c_void],
+        "dd_moe_tokens_prepare": [_c_void, _c_void, _c_int],
         "dd_moe_tokens_most": [_c_void],
         "dd_moe_tokens": [_c_void, _c_void, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_int, _c_void, _c_void],
         "dd_mx4_quantize": [_c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_int, _c_void],
@@ -1535,7 +1535,7 @@ class _ExpertLayer(ctypes.Structure):                # csrc/moe_tokens.cu: DdExp
                                        "shared_down", "shared_down_scales", "router", "table", "correction")] + \
                [(n, _c_int) for n in ("kind", "width", "inner", "experts", "top", "vocab", "identity", "gated", "form", "act", "softmax",
                                       "groups", "keep", "renormalize", "weight_input", "shared_inner", "shared_form", "shared_gate",
-                                      "router_stride", "settled")] + \
+                                      "router_stride", "settled", "up_shift", "unit_part", "shared_part")] + \
                [(n, _c_float) for n in ("limit", "alpha", "shared_limit", "shared_alpha", "weight_scale")]
 
 
@@ -1601,7 +1601,7 @@ class ExpertLayer:
             _ptr(correction, "correction"), 2 if four else (0 if self.dtype == torch.float32 else 1), width, inner, E, top,
             table.shape[0] if table is not None else 0, identity, 1 if gated else 0, GATED_FORMS[form], ACTIVATIONS[activation],
             1 if softmax else 0, groups, keep, 1 if renormalize else 0, 1 if weight_input else 0, shared[1].shape[1] if shared else 0,
-            GATED_FORMS[s_form], 1 if shared_gate else 0, router.stride(0) if router is not None else 0, 0, float(limit), float(alpha),
+            GATED_FORMS[s_form], 1 if shared_gate else 0, router.stride(0) if router is not None else 0, 0, 0, 0, 0, float(limit), float(alpha),
             float(s_limit), float(s_alpha), float(weight_scale) / (top if table is not None else 1))
         self.device_index = gate_up.device.index
         if any(t is not None and t.device.index != self.device_index for t in (router, table, correction)) or \
@@ -1610,7 +1610,7 @@ class ExpertLayer:
         self._at = ctypes.addressof(raw)
         self._map_store = ctypes.create_string_buffer(512 + 64)      # the matrices as TMA takes them, at a 64-byte boundary
         self._maps = (ctypes.addressof(self._map_store) + 63) // 64 * 64
-        _call(library("core"), "dd_moe_tokens_maps", self._at, self._maps, n_kernels=0)
+        _call(library("core"), "dd_moe_tokens_prepare", self._at, self._maps, sm_count(gate_up.device), n_kernels=0)
         # rows so wide that they do not fit into shared memory beside the rings go to the kernels of larger steps
         self.most_tokens = int(library("core").dd_moe_tokens_most(self._at))
         if settled and not torch.cuda.is_current_stream_capturing():         # (nothing is waited for in a capture)
@@ -1629,7 +1629,8 @@ def moe_tokens(layer, y, residual=None, ids=None, out=None):
     chosen units, the shared unit, the weighted sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the
     layer's dtype; ids int32 [T] for a layer by table; out float32 (residual itself may be given). Sums are float32; a hidden row meets
     the down matrix as float32, in bfloat16 layers as the sum of three bfloat16 numbers (24 bits). 4-bit layers: y's elements are kept
-    exactly down to 2^-31 of their row's largest and to 2^-39 of it below that. An expert or token id out of range sets error bit 1 and is left out."""
+    exactly down to 2^-31 of their row's largest and to 2^-39 of it below that. A token has the same bits alone and beside any others.
+    An expert or token id out of range sets error bit 1 and is left out."""
     T = y.shape[0]
     if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > layer.most_tokens:
         raise KernelError(f"moe_tokens: rows {tuple(y.shape)} {y.dtype} do not fit a layer of width {layer.width} {layer.dtype} "

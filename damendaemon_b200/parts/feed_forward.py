@@ -4,7 +4,8 @@ table of token ids: small gated units, a token's chosen ones weighted equally, a
 token; their products run grouped, expert by expert, over rows sorted on the device. Experts chosen
 by a router's scores: the same grouped products after a routing kernel, each chosen expert's output, or its input, weighted
 by its score; the experts are gated units or plain ones of two matrices. 'gated': one dense gated unit. 'none': a layer without a feed-forward.
-A step of a few tokens runs a whole expert layer in two kernels. With the runtime's ``feed_forward`` 'mx4' every matrix of a
+A step of a few tokens runs a whole expert layer in two kernels, in which a token has the same bits alone and beside any others (they
+may change where a step is too large for these, within the error of the sums' order). With the runtime's ``feed_forward`` 'mx4' every matrix of a
 feed-forward becomes microscaled 4-bit numbers when the part is built (the router stays as it is)."""
 from __future__ import annotations
 
@@ -49,7 +50,7 @@ def _check_held(runtime, tensor_cores, width, inner):
 
 def _few_tokens(runtime, gate_up, down, **options):
     """The layer as kernels.moe_tokens takes it, or None where the kernels of larger steps serve these too: a runtime that
-    wants the kernels whose rows do not depend on what is beside them, float32 matrices of a size whose products keep a row's
+    wants the kernels whose rows have the same bits in a step of any size, float32 matrices of a size whose products keep a row's
     bits for the same reason (splits_float32), or more experts than a block chooses among."""
     if runtime.gemm == "simt" or (runtime.dtype == torch.float32 and not splits_float32(*down.shape[1:])) or \
             not kernels.expert_layer_fits(options["top"], gate_up.shape[0] + options.get("identity", 0) + 1):
