@@ -551,6 +551,17 @@ template <int W> struct Barriers {
         tc::fence_proxy_async();
     }
 };
+// The terms of a value beyond bfloat16's largest number: an infinity is the first term alone, a number begins with the largest.
+constexpr float BF16_MAX = 3.38953138925153547590e38f;       // 2^128 - 2^120
+__device__ __noinline__ void put_terms_of_ends(__nv_bfloat16* h, int row, float v) {
+    const __nv_bfloat16 first = isfinite(v) ? __float2bfloat16_rn(copysignf(BF16_MAX, v)) : __float2bfloat16_rn(v);
+    const float rest = isfinite(v) ? v - __bfloat162float(first) : 0.f;
+    const __nv_bfloat16 second = __float2bfloat16_rn(rest);
+    h[0] = first;
+    h[row] = second;
+    h[2 * row] = __float2bfloat16_rn(rest - __bfloat162float(second));
+    static_assert(TERMS == 3, "the terms above");
+}
 // A unit's value, in float32, as its hidden row keeps it.
 template <int KIND>
 __device__ __forceinline__ void put_hidden(const Call& c, bool shared, int unit, int t, int feature, float v) {
@@ -559,6 +570,7 @@ __device__ __forceinline__ void put_hidden(const Call& c, bool shared, int unit,
     if constexpr (KIND == F32) reinterpret_cast<float*>(c.hidden)[before + slot * row + feature] = v;
     else {
         __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(c.hidden) + before * TERMS + slot * TERMS * row + feature;
+        if (!(fabsf(v) <= BF16_MAX)) return put_terms_of_ends(h, row, v);
 #pragma unroll
         for (int i = 0; i < TERMS; ++i) {
             const __nv_bfloat16 term = __float2bfloat16_rn(v);
@@ -658,7 +670,8 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
         }
         __syncthreads();
         if (t < c.T) {
-            const int exponent = (int)(r.y_top[t] >> 23), up = exponent == 255 ? 0 : min(126, 141 - exponent);      // times 2^up
+            // times 2^up (where the largest is no number, so far down that no number becomes an infinity beside it)
+            const int up = min(126, 141 - (int)(r.y_top[t] >> 23));
             const float times = __uint_as_float((uint32_t)(up + 127) << 23);
             if (warp % by == 0 && lane == 0) r.y_back[t] = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll 1

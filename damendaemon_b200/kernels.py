@@ -1629,7 +1629,7 @@ def moe_tokens(layer, y, residual=None, ids=None, out=None):
     chosen units, the shared unit, the weighted sum, added to ``residual`` (float32 [T, width]; None: to nothing). y [T, width] in the
     layer's dtype; ids int32 [T] for a layer by table; out float32 (residual itself may be given). Sums are float32; a hidden row meets
     the down matrix as float32, in bfloat16 layers as the sum of three bfloat16 numbers (24 bits). 4-bit layers: y's elements are kept
-    exactly down to 2^-31 of their row's largest and to 2^-39 of it below that. A token has the same bits alone and beside any others.
+    exactly down to 2^-31 of their row's largest and to 2^-39 of it below that, and hidden values beyond 2^120 may come out infinite. A token has the same bits alone and beside any others.
     An expert or token id out of range sets error bit 1 and is left out."""
     T = y.shape[0]
     if y.dim() != 2 or y.stride(1) != 1 or y.shape[1] != layer.width or y.dtype != layer.dtype or T > layer.most_tokens:
@@ -1739,7 +1739,8 @@ def mx4_values(w, dtype=torch.bfloat16):
 
 def gemm_mx4(a, w, bias=None, residual=None, activation=None, out_dtype=None, out=None):
     """act(a @ w.T + bias) (+ residual), as gemm_tcgen05 with a 4-bit matrix: a [M, K] bfloat16, w an Mx4Matrix [N, K], bias
-    [N] and residual [M, N] float32, out bfloat16 or float32; float32 sums of exact products. Beyond MX4_FUSED_ROWS rows the matrix becomes bfloat16 first, which loses nothing (2,048 x 6,400 x 1,600: 36 us,
+    [N] and residual [M, N] float32, out bfloat16 or float32; float32 sums of exact products. (Up to 32 rows, and in small
+    products, 32 of them are added before their power of two comes in: elements of a beyond 2^120 may come out infinite.) Beyond MX4_FUSED_ROWS rows the matrix becomes bfloat16 first, which loses nothing (2,048 x 6,400 x 1,600: 36 us,
     50 for the best of the kernels that turn codes into rows for every tile: they read X once for 128 features)."""
     _rows(a, "a")
     M, K = a.shape
