@@ -102,6 +102,8 @@ class Engine:
         # float32 products on the tensor cores first write their tokens in parts: the widest of them counts
         self._plane_width = max((t.shape[1] for t in weights.values() if self.dtype == torch.float32 and gemm != "simt" and t.dim() == 2
                                  and splits_float32(*t.shape)), default=0)
+        # a product with a 4-bit matrix makes it a bfloat16 one where a step's rows are many: the largest of them counts
+        self._unpacked_bytes = max((2 * t.shape[0] * t.shape[1] for t in weights.values() if isinstance(t, kernels.Mx4Matrix) and t.dim() == 2), default=0)
         self._admit_memory()
         self.cache.allocate(self.device, self.dtype)
         self._caches = [self.cache.layer_view(i) if e.cache_of is None else self.cache.layer_view(e.cache_of, writable=False)
@@ -151,9 +153,13 @@ class Engine:
         per_token = 4 * self.spec.width * 4 + (3 * self.spec.width + widest) * element
         tokens = min(self.max_context * self.cache.max_requests, 8192)
         self.workspace_bytes = workspace = tokens * per_token + self.cache.max_requests * self.spec.vocab_size * 4 + \
-            kernels.gemm_split_plane_bytes(tokens, self._plane_width, 128)
+            kernels.gemm_split_plane_bytes(tokens, self._plane_width, 128) + (self._unpacked_bytes if tokens > kernels.MX4_FUSED_ROWS else 0)
         free, total = torch.cuda.mem_get_info(self.device)
         need = cache_bytes + workspace + self.HEADROOM_BYTES
+        if need > free:
+            # matrices that the parts joined or quantised are free again, but not before torch's allocator gives their memory back
+            torch.cuda.empty_cache()
+            free, total = torch.cuda.mem_get_info(self.device)
         if need > free:
             gib = lambda b: f"{b / 2 ** 30:.2f} GiB"
             raise MemoryError(f"the cache needs {gib(cache_bytes)} ({self.kv_tokens} tokens), a step's activations about "
