@@ -1203,11 +1203,21 @@ UpPlan plan_up(const DdExpertLayer& l, int T) {
     u.stage = UP_WARPS * S::STAGE_BYTES;
     return u;
 }
+// up_kernel's tiles, at most, in a call of T tokens: they, and the matrices' rows, are counted in fewer than 32 bits.
+int units_of(const DdExpertLayer& l, int T) { return T * l.top < l.experts ? T * l.top : l.experts; }
+template <int KIND> long long most_tiles(const DdExpertLayer& l, int T) {
+    using S = Stream<KIND>;
+    const int features = l.gated ? S::HALF : S::ROWS;
+    return (long long)units_of(l, T) * ((l.inner + features - 1) / features) + (l.shared_inner + S::HALF - 1) / S::HALF;
+}
+template <int KIND> bool counts_fit(const DdExpertLayer& l, int T) {
+    return most_tiles<KIND>(l, T) <= (1 << 21) && (long long)l.experts * l.inner * 2 <= INT_MAX && (long long)l.experts * l.width <= INT_MAX;
+}
 template <int KIND>
 int most_tokens(const DdExpertLayer& l) {        // with two stages a ring
     for (int T = MAX_TOKENS; T > 0; --T) {
         const UpPlan u = plan_up<KIND>(l, T);
-        if (u.fixed + 2 * u.stage <= MOST_SHARED) return T;
+        if (u.fixed + 2 * u.stage <= MOST_SHARED && counts_fit<KIND>(l, T)) return T;
     }
     return 0;
 }
@@ -1228,10 +1238,8 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     c.stages = (int)((MOST_SHARED - u.fixed) / u.stage);
     if (c.stages > S::MOST_STAGES) c.stages = S::MOST_STAGES;
     const int most = up_blocks(c.cluster, sms);
-    const int features = c.l.gated ? S::HALF : S::ROWS;
-    const long long at_most = (long long)c.max_units * ((c.l.inner + features - 1) / features) + (c.l.shared_inner + S::HALF - 1) / S::HALF;
-    if (at_most > (1 << 21) || (long long)c.l.experts * c.l.inner * 2 > INT_MAX || (long long)c.l.experts * c.l.width > INT_MAX)
-        return dd_fail("dd_moe_tokens: %d experts of %d x %d are too large", c.l.experts, c.l.inner, c.l.width);
+    if (!counts_fit<KIND>(c.l, c.T)) return dd_fail("dd_moe_tokens: %d experts of %d x %d are too large", c.l.experts, c.l.inner, c.l.width);
+    const long long at_most = most_tiles<KIND>(c.l, c.T);
     const int blocks = at_most < most ? (int)((at_most + c.cluster - 1) / c.cluster * c.cluster) : most;
     if (int e = launch_up<KIND>(c, m, blocks, u.fixed + c.stages * u.stage, s)) return e;
     c.shares = shares_of(c.l, S::STEP, shared_weight(KIND, c.T));
@@ -1298,14 +1306,14 @@ int hidden_row(int kind, int inner) { return (inner + step_of(kind) - 1) / step_
 size_t hidden_bytes(const DdExpertLayer& l, int T, int max_units) {
     return (size_t)T * (l.kind == F32 ? 4 : 2 * TERMS) * ((size_t)max_units * hidden_row(l.kind, l.inner) + hidden_row(l.kind, l.shared_inner));
 }
-int units_of(const DdExpertLayer& l, int T) { return T * l.top < l.experts ? T * l.top : l.experts; }
 }  // namespace
 
 // Bytes of scratch that a call of T tokens needs (16-byte aligned).
 DD_API long long dd_moe_tokens_scratch(const DdExpertLayer* l, int T) {
     return (long long)(sizeof(Plan) + hidden_bytes(*l, T, units_of(*l, T)));
 }
-// The most tokens that a call with this layer can take (its rows have to fit into shared memory beside the rings).
+// The most tokens that a call with this layer can take (its rows have to fit into shared memory beside the rings, its tiles to be
+// counted); 0: the layer is for the kernels of larger steps.
 DD_API int dd_moe_tokens_most(const DdExpertLayer* l) {
     return l->kind == F32 ? most_tokens<F32>(*l) : l->kind == BF16 ? most_tokens<BF16>(*l) : most_tokens<MX4>(*l);
 }
