@@ -55,8 +55,8 @@ class Runtime:
     gemm: str = "auto"            # 'auto' | 'simt' | 'tcgen05'
     attention: str = "auto"       # 'auto' | 'mma' (no tcgen05 prompt kernel) | 'rows' (the general kernel only)
     attention_tuning: AttentionTuning = field(default_factory=AttentionTuning)   # measured thresholds of the kernel choice
-    feed_forward: str = "auto"    # 'auto' (matrices of feed-forwards in the engine dtype) | 'mx4' (in microscaled 4-bit numbers)
     page_size: int = 16           # tokens per cache page (mixers ask their kernels what they support at this size)
+    feed_forward: str = "auto"    # 'auto' (matrices of feed-forwards in the engine dtype) | 'mx4' (in microscaled 4-bit numbers)
 
 
 class Part:
