@@ -35,9 +35,6 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int k, int n, b
     return *reinterpret_cast<const uint4*>(row + k);
 }
 
-// Asks L2 for the line of an address, whatever wrote it: no value is taken, so it may stand before dd_grid_wait where a load may not.
-__device__ __forceinline__ void ask_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at) : "memory"); }
-
 // ---------------------------------------------------------------- a warp's share of a product, 16 rows of W by eight rows of X
 // W bfloat16: steps of 32 k, two instructions each, AHEAD steps requested at a time. w0, w1: rows g and g + 8 of W; x: row g of X
 // (whole 16-byte pieces). `have` holds what Ahead::load fetched of the first steps, before X was there. (For matrices of a few rows, which
@@ -52,16 +49,6 @@ struct Ahead {
             const int k = from + u < to ? (from + u) * 32 + t8 : K;       // past the share: zeros
             a0[u] = load8(w0, k, K, wide);
             a1[u] = load8(w1, k, K, wide);
-        }
-    }
-    static __device__ __forceinline__ void ask(const __nv_bfloat16* w0, const __nv_bfloat16* w1, int K, int from, int to) {
-        const int t8 = (threadIdx.x & 3) * 8;
-#pragma unroll
-        for (int u = 0; u < STEPS; ++u) {
-            const int k = (from + u) * 32 + t8;
-            if (from + u >= to || k >= K) continue;
-            ask_l2(w0 + k);
-            ask_l2(w1 + k);
         }
     }
 };

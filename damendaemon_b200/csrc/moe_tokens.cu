@@ -598,18 +598,14 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, width = c.l.width;
     dd_launch_dependents();
     if (c.l.shared_inner && c.w_wide) ask_for(c.l.shared_gate_up, matrix_bytes(KIND, (size_t)2 * c.l.shared_inner, width));
-    // The warp's first item of the router: of a settled layer it is read while the kernel before this one ends, of another one only asked
-    // into L2, and read behind the wait (one token, sixteen experts of 1,600 x 1,600: 24.6 us settled, 26.0 not).
+    // The warp's first item of the router: of a settled layer it is read while the kernel before this one ends, of another one behind the
+    // wait (one token, sixteen experts of 1,600 x 1,600: 24.6 us settled, 25.3 not).
     few::Ahead ahead;
     auto read_router = [&] {
         const RouterItem it(c, KIND, warp);
         if (it.from < it.to) ahead.load(router_row(c, it.tile, lane >> 2), router_row(c, it.tile, (lane >> 2) + 8), width, it.from, it.to, c.router_wide);
     };
-    if (KIND != F32 && c.l.router) {
-        const RouterItem it(c, KIND, warp);
-        if (c.l.settled) read_router();
-        else few::Ahead::ask(router_row(c, it.tile, lane >> 2), router_row(c, it.tile, (lane >> 2) + 8), width, it.from, it.to);
-    }
+    if (KIND != F32 && c.l.router && c.l.settled) read_router();
     bars.init();
     if (threadIdx.x == 0) {
         if (c.w_wide) tc::prefetch_tensormap(&maps.gate_up);

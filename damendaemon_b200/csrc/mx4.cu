@@ -163,19 +163,10 @@ gemm_mx4_rows_kernel(const RowsParams p) {
         }
     };
     dd_launch_dependents();
-    // A settled matrix is read while the kernel before this one ends; of one that this kernel may have made the first codes and scales are
-    // only asked into L2, and read behind its end, with the rows (6,400 x 1,600, one row, in a graph: 4.65 us settled, 5.2 not).
+    // A settled matrix is read while the kernel before this one ends, one that this kernel may have made behind its end, with the rows
+    // (6,400 x 1,600, one row, in a graph: 4.65 us settled, 4.85 not; from memory 4.9 and 5.4. Asking L2 for the first codes before the wait instead
+    // takes longer than either, 5.7).
     if (p.settled) fetch(first);
-    else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = min(first + u, p.groups - 1);
-            few::ask_l2(w0 + at * 4);
-            few::ask_l2(w1 + at * 4);
-            few::ask_l2(s0 + at);
-            few::ask_l2(s1 + at);
-        }
-    }
     dd_grid_wait();
     if (!p.settled) fetch(first);
     const __nv_bfloat16* x[NT];
