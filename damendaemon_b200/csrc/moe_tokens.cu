@@ -16,7 +16,7 @@
 //
 // A token's bits do not depend on what is beside it, nor on how many tokens are: a row of a matrix is cut into parts by the layer alone
 // (DdExpertLayer: up_shift, unit_part, shared_part), a part is one sum from its first product to its last, and the parts' sums are
-// added in one order, whichever warps had them. How many parts a warp takes is free to follow the step's work.
+// added in one order, whichever warps had them. How many parts a warp of down_kernel takes is free to follow the step's work.
 //
 // Weights go to mma.sync (float32: to multiply-adds) through a ring of TMA boxes that every warp has for itself and that runs ahead
 // over the ends of its tiles: a warp waits for nobody but its own weights, and one lane asks for them (with cp.async, a lane's
@@ -41,7 +41,7 @@ struct DdExpertLayer {
     int softmax, groups, keep, renormalize, weight_input;
     int shared_inner, shared_form, shared_gate, router_stride;
     int settled;                 // no kernel that is still running writes the router
-    int up_shift;                // a gate or up row's sum: 2^up_shift parts
+    int up_shift;                // a gate or up row's sum: 2^up_shift parts, each of a warp of its own
     int unit_part, shared_part;  // a down row's: steps of a part (the last may have fewer), of an expert's and of the shared unit's
     float limit, alpha, shared_limit, shared_alpha, weight_scale;
 };
@@ -109,29 +109,6 @@ struct Maps { CUtensorMap gate_up, shared_gate_up, down, shared_down; };
 
 struct Tile { float sum[16][few::COLUMNS + 1]; };
 template <int N> struct Count { static constexpr int value = N; };
-
-// Sums of parts that come one after the other, added as the leaves of a binary tree: call number j (from 0) with the j-th part's; where
-// j + 1 is a power of two the result is the sum of all so far. A subtree's sum does not depend on who made it.
-template <int LEVELS>
-__device__ __forceinline__ float tree_add(float* level, int j, float v) {
-    bool more = true;
-#pragma unroll
-    for (int l = 0; l < LEVELS; ++l)
-        if (more) {
-            if (j >> l & 1) v = level[l] + v;
-            else { level[l] = v; more = false; }
-        }
-    return v;
-}
-// ... of x(0), ..., x(n - 1), n a power of two above one.
-template <typename X>
-__device__ __forceinline__ float tree_sum(int n, X x) {
-    float sum = 0.f, level[3];
-#pragma unroll 1
-    for (int j = 0; 2 * j < n; ++j) sum = tree_add<3>(level, j, x(2 * j) + x(2 * j + 1));
-    return sum;
-}
-constexpr int TREE = 2;                          // a warp takes up to 2^TREE parts of a tile of up_kernel
 
 // What a warp multiplies at a time, a tile: 16 rows of a matrix on mma.sync, 4 with multiply-adds. A stage of its ring is one TMA box
 // of a tile, gate and up rows together (a copy has a cost of its own: eight tokens with eight each of 64 experts of 2 x 1,024 x 2,048, 4 bits:
@@ -702,16 +679,9 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     const int per_unit = (c.l.inner + features - 1) / features, for_shared = (c.l.shared_inner + S::HALF - 1) / S::HALF;
     const int total = for_shared + r.n_units * per_unit;
     const float per_unit_inverse = 1.0f / (float)per_unit;
-    // `share` warps share a tile's columns: as few as give most warps a tile (with more tiles than warps the last round's are spread
-    // over the SMs, and enough of them to keep the memory busy; a tile alone in a warp needs no barrier of the block)
-    // (each of them takes as many of the columns' parts, at most four, so that their sums make the same tree)
-    const int warps = gridDim.x * UP_WARPS;
-    int share_shift = max(0, c.l.up_shift - TREE);
-    while (share_shift < c.l.up_shift && (total << share_shift) * 4 < warps * 3) ++share_shift;
-    const int share = 1 << share_shift, own_shift = c.l.up_shift - share_shift;
-    const int slots = UP_WARPS >> share_shift, slot = warp >> share_shift, part = warp & (share - 1), stride = gridDim.x * slots;
-    const int steps = (width + S::STEP - 1) / S::STEP, from = steps * part >> share_shift, to = steps * (part + 1) >> share_shift;
-    auto part_end = [&](int j) { return steps * ((part << own_shift) + j + 1) >> c.l.up_shift; };       // of the warp's j-th part
+    // `share` warps share a tile's columns (choose_parts; a tile alone in a warp needs no barrier of the block)
+    const int share = 1 << c.l.up_shift, slots = UP_WARPS >> c.l.up_shift, slot = warp >> c.l.up_shift, part = warp & (share - 1), stride = gridDim.x * slots;
+    const int steps = (width + S::STEP - 1) / S::STEP, from = steps * part >> c.l.up_shift, to = steps * (part + 1) >> c.l.up_shift;
     // a tile: its unit (-1: the shared one), first feature, matrix of the stack (gate and up are two), and the rows where its halves begin:
     // gate rows and the same features' up rows; plain: neighbours
     struct Place { int unit, first, matrix, row_a, row_b; };
@@ -775,18 +745,13 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 by_count(__popc(users), [&](auto count) {
                     constexpr int N = decltype(count)::value;
                     const uint32_t list = list_of(users);         // (what it lacks to N names token 0 again, and is dropped)
-                    float level[TREE], sum = 0.f;
-#pragma unroll 1
-                    for (int j = 0, s = from; !(j >> own_shift); ++j) {
-                        unsigned long long d[few::F32_ROWS][N] = {};
-                        for (const int end = part_end(j); s < end; ++s) {
-                            fma_step<N>(next(s), reinterpret_cast<const float*>(y), c.y_pitch / 4, list, s, d);
-                            __syncwarp();
-                            fetch();      // into the stage before this one, which the warp has read
-                        }
-                        sum = tree_add<TREE>(level, j, row_sums<N>(d));
+                    unsigned long long d[few::F32_ROWS][N] = {};
+                    for (int s = from; s < to; ++s) {
+                        fma_step<N>(next(s), reinterpret_cast<const float*>(y), c.y_pitch / 4, list, s, d);
+                        __syncwarp();
+                        fetch();          // into the stage before this one, which the warp has read
                     }
-                    put_rows<N>(red[turn][warp], 0, list, __popc(users), sum);
+                    put_rows<N>(red[turn][warp], 0, list, __popc(users), row_sums<N>(d));
                 });
             if (share > 1) __syncthreads();          // (the other set is written next: one barrier a round is enough)
             else __syncwarp();
@@ -795,22 +760,21 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 for (int i = lane; i < n * c.T; i += 32) {
                     const int t = i / n, k = i % n, feature = p.first + k;
                     if (feature >= (shared ? c.l.shared_inner : c.l.inner) || !(users >> t & 1)) continue;
-                    auto sum_of = [&](int row) {
-                        const Tile* have = &red[turn][slot * share];
-                        return share == 1 ? have->sum[row][t] : tree_sum(share, [&](int s) { return have[s].sum[row][t]; });
-                    };
-                    const float a = sum_of(k), b = n == S::HALF ? sum_of(k + S::HALF) : 0.f;
+                    const Tile* have = &red[turn][warp];
+                    const int other = n == S::HALF ? k + S::HALF : k;         // (of a plain unit nobody looks at b)
+                    float a = have->sum[k][t], b = have->sum[other][t];
+#pragma unroll 1
+                    for (int s = 1; s < share; ++s) {
+                        a += have[s].sum[k][t];
+                        b += have[s].sum[other][t];
+                    }
                     put_hidden<KIND>(c, shared, p.unit, t, feature, unit_value(c, shared, a, b, shared ? r.gate[t] : r.unit_weight[p.unit][t]));
                 }
             }
         } else {
-            float d[1][4] = {}, level[4][TREE];
-            if (mine)
-#pragma unroll 1
-              for (int j = 0, s = from; !(j >> own_shift); ++j) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[0][i] = 0.f;
-                for (const int end = part_end(j); s < end; ++s) {
+            float d[1][4] = {};
+            if (mine) {
+                for (int s = from; s < to; ++s) {
                     const uint32_t at = next(s);
 #pragma unroll
                     for (int sub = 0; sub < S::SUB; ++sub) {
@@ -831,24 +795,16 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                     __syncwarp();
                     fetch();
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[0][i] = tree_add<TREE>(level[i], j, d[0][i]);
-              }
+            }
             if (share > 1) {                      // the first of the sharers adds up
-                put_tile<KIND>(red[turn][warp], d[0]);
+                if (part) put_tile<KIND>(red[turn][warp], d[0]);
                 __syncthreads();
                 if (mine && part == 0) {
                     const int g = row_of<KIND>(lane >> 2), t = lane & 3;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d[0][i] = 0.f;
-                    float level_of[4][3];
 #pragma unroll 1
-                    for (int j = 0; 2 * j < share; ++j)
+                    for (int s = 1; s < share; ++s)          // (its own part's are still here)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int row = g + 8 * (i >> 1), column = 2 * t + (i & 1);
-                            d[0][i] = tree_add<3>(level_of[i], j, red[turn][warp + 2 * j].sum[row][column] + red[turn][warp + 2 * j + 1].sum[row][column]);
-                        }
+                        for (int i = 0; i < 4; ++i) d[0][i] += red[turn][warp + s].sum[g + 8 * (i >> 1)][2 * t + (i & 1)];
                 }
             }
             if (mine && part == 0) {
@@ -873,9 +829,13 @@ up_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
     if (bars.gave_up && lane == 0) atomicOr(c.error_flag, 8);
 }
 
-// A step of the shared unit, which every token uses, takes longer with three times eight columns, whose pieces there are no registers to
-// ask for ahead (eight tokens, 2,048 x 2,048 and a shared unit 82.4 -> 71.8 us).
-__host__ __device__ constexpr int shared_weight(int kind, int T) { return kind == F32 || T * TERMS <= 2 * few::COLUMNS ? 4 : kind == BF16 ? 12 : 5; }
+// A step of the shared unit, which every token uses, takes longer than an expert's, in quarters of which this is: in bfloat16 layers with three
+// times eight columns, whose pieces there are no registers to ask for ahead (eight tokens, 2,048 x 2,048 and a shared unit, 4: 92.0 us, 12: 74.3),
+// in float32 ones with more than four tokens, for the same reason (1,600 x 1,600 and a shared unit, 4: 113.6 us, 16: 103.0).
+__host__ __device__ constexpr int shared_weight(int kind, int T) {
+    const int columns = (T * TERMS + few::COLUMNS - 1) / few::COLUMNS;
+    return kind == F32 ? (T == 1 ? 4 : T == 2 ? 5 : T <= 4 ? 8 : 16) : kind == BF16 ? (columns == 1 ? 4 : columns == 2 ? 6 : 12) : columns < 3 ? 4 : 6;
+}
 
 // The sums of a part's columns on their way from the instruction's registers to their tokens.
 struct Columns { float sum[16][TERMS * MAX_TOKENS + 1]; };
@@ -979,7 +939,10 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                 const float* x = reinterpret_cast<const float*>(c.hidden) + hidden;
                 float4 b[AT_ONCE<N>];             // up to four rows' next step (they come from L2)
                 if constexpr (N <= 4) take_rows<N>(b, x, ld, list, at - begin, 0);
-                for (int s = at, j = first_j; s < end; ++j) {
+                const int which = lane * (few::F32_ROWS * N) / 32;
+                const bool owner = owns_sum<N>(n);
+                float* own_sum = place_of(owner ? which % N : 0, first_j) + which / N;
+                for (int s = at; s < end; own_sum += S::ROWS) {
                     unsigned long long d[few::F32_ROWS][N] = {};
                     for (const int stop = min(s + part, end); s < stop; ++s) {
                         if constexpr (N <= 4) {
@@ -993,8 +956,7 @@ down_kernel(const __grid_constant__ Call c, const __grid_constant__ Maps maps) {
                         fetch();
                     }
                     const float sum = row_sums<N>(d);
-                    const int which = lane * (few::F32_ROWS * N) / 32;
-                    if (owns_sum<N>(n)) place_of(which % N, j)[which / N] = sum;
+                    if (owner) *own_sum = sum;
                 }
             });
         else {
@@ -1245,12 +1207,14 @@ int launch_both(Call& c, const Maps& m, int sms, cudaStream_t s) {
     return warps == 16 ? launch_down<KIND, 16>(c, m, s) : warps == 8 ? launch_down<KIND, 8>(c, m, s) : launch_down<KIND, 4>(c, m, s);
 }
 
-// How many parts the sums of a row are cut into, by the layer alone. up_kernel: the warps that one token's step wants on a tile.
-// down_kernel: the lengths of parts, of a unit and of the shared unit, that on average leave the warps of a block the least to do one after
-// the other in steps of one to eight tokens (with as many experts as so many tokens choose on average), counting what a part costs
+// How many parts the sums of a row are cut into, by the layer alone. up_kernel: as few warps on a tile as give at least three eighths of the
+// grid's warps one in a step of one token (one token and eight of 1,600 x 1,600, two of sixteen experts and a shared unit: 21.2 and 49.8 us with
+// two warps, 24.9 and 51.9 with one, 22.9 and 51.2 with four; one and eight of 64 4-bit experts, eight a token, 27.7 and 80.9 with one, 27.2 and 86.5
+// with two). down_kernel: the lengths of parts, of a unit and of the shared unit, that on average leave the warps of a block the least to do
+// one after the other in steps of one to eight tokens (with as many experts as so many tokens choose on average), counting what a part costs
 // beside its steps: its sums go through shared memory. Of eleven layers timed at 1, 2, 4 and 8 tokens with other lengths the ones taken are
-// within 1.5 % of the best on average. (Cut wherever a warp's share ends, a token's bits would depend on its neighbours' experts: one token of
-// 1,600 x 1,600 24.7 us, now 23.9; eight tokens, 2,048 x 2,048 and a shared unit 70.0 and 70.9; five of the float32 layer of plain units 49.8 and 51.3.)
+// within 1.5 % of the best on average. (Cut by a step's own work, a token's bits would depend on its neighbours' experts; one token of
+// 1,600 x 1,600 24.7 us, now 22.6; eight, 2,048 x 2,048 and a shared unit, 70.0 and 68.4; five of the float32 layer of plain units 49.8 and 50.0.)
 template <int KIND>
 void choose_parts(DdExpertLayer& l, int sms) {
     using S = Stream<KIND>;
@@ -1258,10 +1222,10 @@ void choose_parts(DdExpertLayer& l, int sms) {
     const long long tiles = (l.shared_inner + S::HALF - 1) / S::HALF + (long long)least * ((l.inner + features - 1) / features);
     const int warps = up_blocks(plan_up<KIND>(l, 1).cluster, sms) * UP_WARPS, steps = dd_ceil_div(l.width, S::STEP);
     l.up_shift = 0;
-    while ((UP_WARPS >> l.up_shift) > 1 && (2 << l.up_shift) <= steps && (tiles << l.up_shift) * 4 < warps * 3) ++l.up_shift;
+    while ((UP_WARPS >> l.up_shift) > 1 && (2 << l.up_shift) <= steps && (tiles << l.up_shift) * 8 < warps * 3) ++l.up_shift;
 
     const int W = down_warps<KIND>(l, sms), unit_steps = dd_ceil_div(l.inner, S::STEP), shared_steps = dd_ceil_div(l.shared_inner, S::STEP);
-    const int beside = KIND == BF16 ? 4 : KIND == MX4 ? 1 : 2;        // quarters of a step
+    const int beside = KIND == MX4 ? 1 : 2;      // quarters of a step
     double best = 1e30;
     for (int p = 32, last_p = 0; p > 0; --p) {    // (about) that many parts of a unit, q of the shared one
         DdExpertLayer with = l;
